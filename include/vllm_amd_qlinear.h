@@ -260,6 +260,52 @@ int vaq_fp8_quant_scaled_mm(const void* x, int64_t ldx, const float* x_scale, co
                             int64_t sb_count, const void* bias, void* out, int64_t ldc, int dtype, int64_t size_m,
                             int64_t size_n, int64_t size_k, void* stream);
 
+/*
+ * FP8 (OCP e4m3fn) quantisation in groups of 128 consecutive values of a row (the last group of a row may be shorter), the activations' side of
+ * vaq_fp8_block_scaled_mm:  s = max(max|y| of the group, 1e-10) / 448,  code = e4m3(y / s).  NaN and infinities: a group with a NaN gets a scale and codes of
+ * NaN; one with an infinity an infinite scale, NaN for the infinities and 0 for the rest.
+ *   scales  fp32, that of row r and group g at scales[r * scale_row_stride + g * scale_group_stride]
+ *   out     codes, row stride out_row_stride;  rows of `in` in_row_stride elements apart, unit column stride
+ * vaq_fp8_group_quant              y = in (F16 / BF16 / F32)
+ * vaq_silu_and_mul_fp8_group_quant y = silu(in[r, i]) * in[r, d + i], in fp32 (F16 / BF16; rows of 2 d values, codes and scales of d)
+ * vaq_rms_norm_fp8_group_quant     y = x * rsqrt(mean(x^2) + epsilon) * weight, in fp32, x = input (+ residual), out contiguous.  residual and residual_out are both NULL
+ *                                  or both [tokens, hidden] contiguous and may be the same memory: residual_out = x rounded to the type.  hidden up to 65536.
+ */
+int vaq_fp8_group_quant(const void* in, int in_dtype, int64_t in_row_stride, uint8_t* out, int64_t out_row_stride, float* scales,
+                        int64_t scale_row_stride, int64_t scale_group_stride, int64_t rows, int64_t hidden, void* stream);
+int vaq_silu_and_mul_fp8_group_quant(const void* in, int dtype, int64_t in_row_stride, uint8_t* out, int64_t out_row_stride, float* scales,
+                                     int64_t scale_row_stride, int64_t scale_group_stride, int64_t rows, int64_t d, void* stream);
+int vaq_rms_norm_fp8_group_quant(uint8_t* out, float* scales, int64_t scale_row_stride, int64_t scale_group_stride, const void* input,
+                                 int64_t in_row_stride, const void* weight, float epsilon, const void* residual, void* residual_out, int dtype,
+                                 int64_t tokens, int64_t hidden, void* stream);
+
+/*
+ * FP8 GEMM with a scale for each block of 128:
+ *   out[m, n] = round( sum over blocks kb of  sa[m, kb] * sb[kb, n / 128] * (sum over k in kb of a[m, k] b[k, n])  + bias[n] ),   sums in fp32, one rounding
+ *   a     e4m3fn [M, K] row-major, row stride lda bytes;  b  e4m3fn [K, N] column-major, element (k, n) at b[n * ldb + k]   (lda, ldb multiples of 16, up to 4 MiB)
+ *   sa    fp32, that of row m and block kb at sa[m * sa_row_stride + kb * sa_block_stride]
+ *   sb    fp32, that of block kb of K and nb of N at sb[kb * sb_k_stride + nb * sb_n_stride]
+ *   bias  [N] of the type of out or NULL;  out [M, N] F16 / BF16, 8-byte aligned, row stride ldc elements (a multiple of 4)
+ * K and N are multiples of 16; their last blocks may be shorter than 128.  No scratch.
+ */
+int vaq_fp8_block_scaled_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb, const float* sa, int64_t sa_row_stride,
+                            int64_t sa_block_stride, const float* sb, int64_t sb_k_stride, int64_t sb_n_stride, const void* bias, void* out,
+                            int64_t ldc, int out_dtype, int64_t size_m, int64_t size_n, int64_t size_k, void* stream);
+
+/*
+ * RMSNorm of every query and key head of a qkv projection's result and the rotation by the token's position:
+ *   y = x * rsqrt(mean(x^2 of the head) + epsilon) * weight,  then (u, v) -> (u cos - v sin, v cos + u sin) over pairs of the first rotary_dim values, in fp32, one rounding
+ *   qkv        F16 / BF16, rows qkv_row_stride elements apart: heads_q * head_dim values of queries, heads_k * head_dim of keys, then anything
+ *   q_out      [tokens, heads_q * head_dim], k_out [tokens, heads_k * head_dim], contiguous;  q_weight, k_weight [head_dim]; all of them and qkv's rows 16-byte aligned
+ *   cos_sin    [cos_sin_rows, rotary_dim] F32 or of the type of qkv: rotary_dim / 2 cosines, then as many sines of each position
+ *   positions  int64 [tokens]; a token whose position is not in 0 .. cos_sin_rows - 1 (padding) leaves its rows of q_out and k_out as they are
+ *   interleaved  0: pairs (i, i + rotary_dim / 2), rotary_dim a multiple of 16; 1: pairs (2 i, 2 i + 1)
+ * head_dim is a multiple of 8 up to 512.
+ */
+int vaq_qk_norm_rope(const void* qkv, int64_t qkv_row_stride, void* q_out, void* k_out, int64_t heads_q, int64_t heads_k, int64_t head_dim,
+                     float epsilon, const void* q_weight, const void* k_weight, const void* cos_sin, int cos_sin_dtype, int64_t cos_sin_row_stride,
+                     int64_t cos_sin_rows, int64_t rotary_dim, int interleaved, const int64_t* positions, int dtype, int64_t tokens, void* stream);
+
 #pragma GCC visibility pop
 
 #ifdef __cplusplus

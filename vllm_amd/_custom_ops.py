@@ -666,6 +666,177 @@ def _silu_and_mul_quant_impl(result: torch.Tensor, input: torch.Tensor, scale: t
                                                   d, _stream(input.device)))
 
 
+# ============================================================================ FP8 in groups and blocks of 128
+
+FP8_GROUP = 128
+
+
+def _check_group_size(who: str, group_size: int) -> None:
+    if group_size != FP8_GROUP:
+        raise NotImplementedError(f"{who}: group_size = {group_size} is not built for gfx950 (only {FP8_GROUP})")
+
+
+def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
+    """(rows, row stride) of ``[..., columns]`` with unit column stride and rows one stride apart; None if it is not that."""
+    if t.dim() < 1 or t.numel() == 0:
+        return (0, 0) if t.dim() else None
+    if t.stride(-1) != 1 and t.size(-1) != 1:
+        return None
+    if t.dim() == 2:
+        return t.size(0), t.stride(0)
+    rows = t.numel() // t.size(-1)
+    if t.dim() == 1:
+        return 1, t.size(-1)
+    return (rows, t.size(-1)) if t.is_contiguous() else None
+
+
+def _check_group_quant(who: str, result: torch.Tensor, input: torch.Tensor, scale: torch.Tensor, columns: int,
+                       types: tuple) -> tuple[int, int]:
+    """Checks that the group quantisers share; returns (rows, row stride) of ``input``."""
+    _check(input.is_cuda and result.is_cuda and scale.is_cuda, lambda: f"{who}: tensors must be on GPU")
+    _check(result.device == input.device and scale.device == input.device, lambda: f"{who}: tensors are on different devices")
+    _check(input.dtype in types, lambda: f"{who}: unsupported input dtype {input.dtype}")
+    _check(result.dtype == FP8_DTYPE, lambda: f"{who}: result must be {FP8_DTYPE}")
+    rows = _rows_of(input)
+    _check(rows is not None, lambda: f"{who}: input must be [..., columns] with contiguous columns and rows one stride apart")
+    _check(tuple(result.shape) == (*input.shape[:-1], columns), lambda: f"{who}: result of shape {tuple(result.shape)} does not fit the input")
+    groups = -(-columns // FP8_GROUP)
+    _check(scale.dtype == torch.float32 and scale.dim() == 2 and (rows[0] == 0 or tuple(scale.shape) == (rows[0], groups)),
+           lambda: f"{who}: scale must be float32 [{rows[0]}, {groups}], one for each group of {FP8_GROUP}")
+    return rows
+
+
+def _result_stride(who: str, result: torch.Tensor) -> int:
+    rows = _rows_of(result)
+    _check(rows is not None, lambda: f"{who}: result must have contiguous columns and rows one stride apart")
+    return rows[1]
+
+
+def _group_quant_impl(result: torch.Tensor, input: torch.Tensor, scale: torch.Tensor) -> None:
+    who = "scaled_fp8_group_quant"
+    rows, stride = _check_group_quant(who, result, input, scale, input.size(-1) if input.dim() else 0,
+                                      (torch.float16, torch.bfloat16, torch.float32))
+    if rows == 0:
+        return
+    lib = _lib.load()
+    with _on(input.device):
+        _lib.check(lib.vaq_fp8_group_quant(_ptr(input), _dtype_tag(input.dtype), stride, _ptr(result), _result_stride(who, result),
+                                           _ptr(scale), scale.stride(0), scale.stride(1), rows, input.size(-1),
+                                           _stream(input.device)))
+
+
+def _silu_group_quant_impl(result: torch.Tensor, input: torch.Tensor, scale: torch.Tensor) -> None:
+    who = "silu_and_mul_group_quant"
+    _check(input.dim() > 0 and input.size(-1) % 2 == 0, f"{who}: the last dimension of input must be even")
+    d = input.size(-1) // 2
+    rows, stride = _check_group_quant(who, result, input, scale, d, (torch.float16, torch.bfloat16))
+    if rows == 0:
+        return
+    lib = _lib.load()
+    with _on(input.device):
+        _lib.check(lib.vaq_silu_and_mul_fp8_group_quant(_ptr(input), _dtype_tag(input.dtype), stride, _ptr(result),
+                                                        _result_stride(who, result), _ptr(scale), scale.stride(0),
+                                                        scale.stride(1), rows, d, _stream(input.device)))
+
+
+def _rms_norm_group_quant_impl(result: torch.Tensor, input: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, epsilon: float,
+                               residual: torch.Tensor | None, residual_out: torch.Tensor | None) -> None:
+    who = "rms_norm_group_quant"
+    hidden = input.size(-1) if input.dim() else 0
+    rows, stride = _check_group_quant(who, result, input, scale, hidden, (torch.float16, torch.bfloat16))
+    _check(result.is_contiguous(), f"{who}: result must be contiguous")
+    _check(weight.is_cuda and weight.device == input.device, f"{who}: tensors must be on one GPU")
+    _check(weight.dtype == input.dtype and weight.numel() == hidden and weight.is_contiguous(),
+           f"{who}: weight must be a contiguous [hidden] tensor of the input's dtype")
+    _check(residual is not None or residual_out is None, f"{who}: residual_out without a residual")
+    if residual_out is None:
+        residual_out = residual
+    for t in (residual, residual_out):
+        _check(t is None or (t.device == input.device and t.dtype == input.dtype and t.is_contiguous() and t.shape == input.shape),
+               f"{who}: residual and residual_out must match input and be contiguous")
+    if rows == 0:
+        return
+    lib = _lib.load()
+    with _on(input.device):
+        _lib.check(lib.vaq_rms_norm_fp8_group_quant(_ptr(result), _ptr(scale), scale.stride(0), scale.stride(1), _ptr(input),
+                                                    stride, _ptr(weight), float(epsilon), _ptr(residual), _ptr(residual_out),
+                                                    _dtype_tag(input.dtype), rows, hidden, _stream(input.device)))
+
+
+def _block_scaled_mm_impl(out: torch.Tensor, a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: torch.Tensor,
+                          bias: torch.Tensor | None) -> None:
+    who = "block_scaled_mm"
+    _check(a.dim() == 2 and b.dim() == 2 and out.dim() == 2, f"{who}: a, b and out must be 2-D")
+    (m, k), n = a.shape, b.size(1)
+    _check(b.size(0) == k and tuple(out.shape) == (m, n),
+           lambda: f"{who}: shape mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}, out {tuple(out.shape)}")
+    _check(all(t is None or t.is_cuda for t in (out, a, b, a_scales, b_scales, bias)), f"{who}: all tensors must be on GPU")
+    _check(all(t is None or t.device == a.device for t in (out, b, a_scales, b_scales, bias)),
+           f"{who}: tensors are on different devices")
+    if a.dtype != FP8_DTYPE or b.dtype != FP8_DTYPE:
+        raise NotImplementedError(f"{who}: only {FP8_DTYPE} x {FP8_DTYPE} is built for gfx950 (got {a.dtype} x {b.dtype})")
+    _check(out.dtype in (torch.float16, torch.bfloat16), f"{who}: out must be float16 or bfloat16")
+    _check(k > 0 and n > 0 and k % 16 == 0 and n % 16 == 0, f"{who}: K and N must be multiples of 16")
+    if m == 0:
+        return
+    _check(a.stride(1) == 1 and out.stride(1) == 1, f"{who}: a and out must be row-major")
+    _check(b.stride(0) == 1, f"{who}: b must be column-major")
+    lda, ldc = (a.stride(0), out.stride(0)) if m > 1 else (k, n)      # (the stride of a single row says nothing)
+    _check(lda % 16 == 0 and b.stride(1) % 16 == 0 and ldc % 4 == 0,
+           f"{who}: a.stride(0) and b.stride(1) must be multiples of 16, out.stride(0) of 4")
+    _check(a.data_ptr() % 16 == 0 and b.data_ptr() % 16 == 0 and out.data_ptr() % 8 == 0,
+           f"{who}: a and b must be aligned to 16 bytes, out to 8")
+    kb, nb = -(-k // FP8_GROUP), -(-n // FP8_GROUP)
+    _check(a_scales.dtype == torch.float32 and b_scales.dtype == torch.float32, f"{who}: scales must be float32")
+    _check(tuple(a_scales.shape) == (m, kb), lambda: f"{who}: a_scales must be [M, K / {FP8_GROUP}] = [{m}, {kb}], not {tuple(a_scales.shape)}")
+    _check(tuple(b_scales.shape) == (kb, nb),
+           lambda: f"{who}: b_scales must be [K / {FP8_GROUP}, N / {FP8_GROUP}] = [{kb}, {nb}], not {tuple(b_scales.shape)}")
+    if bias is not None:
+        _check(bias.dim() == 1 and bias.numel() == n and bias.is_contiguous() and bias.dtype == out.dtype,
+               f"{who}: bias must be contiguous [N] of the output dtype")
+    lib = _lib.load()
+    with _on(a.device):
+        tune = _tuning.current_ref()
+        args = (_ptr(a), lda, _ptr(b), b.stride(1) if n > 1 else k, _ptr(a_scales), a_scales.stride(0), a_scales.stride(1), _ptr(b_scales),
+                b_scales.stride(0), b_scales.stride(1), _ptr(bias), _ptr(out), ldc, _dtype_tag(out.dtype), m, n, k, _stream(a.device))
+        _lib.check(lib.vaq_fp8_block_scaled_mm(*args) if tune is None else lib.vaq_fp8_block_scaled_mm_tuned(*args, tune))
+
+
+# ============================================================================ norms of query and key heads, rotation
+
+def _qk_norm_rope_impl(q: torch.Tensor, k: torch.Tensor, qkv: torch.Tensor, num_heads_q: int, num_heads_k: int, head_dim: int,
+                       epsilon: float, q_weight: torch.Tensor, k_weight: torch.Tensor, cos_sin_cache: torch.Tensor,
+                       positions: torch.Tensor, is_neox: bool = True) -> None:
+    who = "qk_norm_rope"
+    every = (q, k, qkv, q_weight, k_weight, cos_sin_cache, positions)
+    _check(all(t.is_cuda for t in every), f"{who}: tensors must be on GPU")
+    _check(all(t.device == qkv.device for t in every), f"{who}: tensors are on different devices")
+    _check(num_heads_q >= 0 and num_heads_k >= 0 and num_heads_q + num_heads_k > 0 and head_dim > 0, f"{who}: no heads")
+    _check(qkv.dtype in (torch.float16, torch.bfloat16), f"{who}: qkv must be float16 or bfloat16")
+    _check(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.size(1) >= (num_heads_q + num_heads_k) * head_dim,
+           f"{who}: qkv must be [tokens, at least (num_heads_q + num_heads_k) * head_dim] with contiguous columns")
+    tokens = qkv.size(0)
+    for t, heads, name in ((q, num_heads_q, "q"), (k, num_heads_k, "k")):
+        _check(t.dtype == qkv.dtype and tuple(t.shape) == (tokens, heads, head_dim) and t.is_contiguous(),
+               f"{who}: {name} must be contiguous [tokens, heads, head_dim] of qkv's dtype")
+    for t in (q_weight, k_weight):
+        _check(t.dtype == qkv.dtype and t.numel() == head_dim and t.is_contiguous(),
+               f"{who}: weights must be contiguous [head_dim] of qkv's dtype")
+    _check(cos_sin_cache.dim() == 2 and cos_sin_cache.dtype in (torch.float32, qkv.dtype)
+           and (cos_sin_cache.stride(1) == 1 or cos_sin_cache.size(1) <= 1),
+           f"{who}: cos_sin_cache must be [positions, rotary_dim] in float32 or qkv's dtype")
+    _check(positions.dtype == torch.int64 and positions.dim() == 1 and positions.numel() == tokens and positions.is_contiguous(),
+           f"{who}: positions must be contiguous int64 [tokens]")
+    if tokens == 0:
+        return
+    lib = _lib.load()
+    with _on(qkv.device):
+        _lib.check(lib.vaq_qk_norm_rope(_ptr(qkv), qkv.stride(0), _ptr(q), _ptr(k), num_heads_q, num_heads_k, head_dim, float(epsilon),
+                                        _ptr(q_weight), _ptr(k_weight), _ptr(cos_sin_cache), _dtype_tag(cos_sin_cache.dtype),
+                                        cos_sin_cache.stride(0), cos_sin_cache.size(0), cos_sin_cache.size(1), int(not is_neox),
+                                        _ptr(positions), _dtype_tag(qkv.dtype), tokens, _stream(qkv.device)))
+
+
 # ============================================================================ registration
 
 _NS = "vllm_amd"
@@ -711,6 +882,21 @@ _register("silu_and_mul_quant", "(Tensor! result, Tensor input, Tensor scale) ->
           _silu_and_mul_quant_impl, lambda result, input, scale: None)
 _register("cutlass_scaled_mm", "(Tensor! out, Tensor a, Tensor b, Tensor a_scales, Tensor b_scales, Tensor? bias) -> ()",
           _scaled_mm_impl, lambda out, a, b, a_scales, b_scales, bias: None)
+_register("scaled_fp8_group_quant", "(Tensor! result, Tensor input, Tensor! scale) -> ()", _group_quant_impl,
+          lambda result, input, scale: None)
+_register("silu_and_mul_group_quant", "(Tensor! result, Tensor input, Tensor! scale) -> ()", _silu_group_quant_impl,
+          lambda result, input, scale: None)
+_register("rms_norm_group_quant",
+          "(Tensor! result, Tensor input, Tensor weight, Tensor! scale, float epsilon, Tensor(a!)? residual, "
+          "Tensor(b!)? residual_out) -> ()",
+          _rms_norm_group_quant_impl, lambda result, input, weight, scale, epsilon, residual, residual_out: None)
+_register("block_scaled_mm", "(Tensor! out, Tensor a, Tensor b, Tensor a_scales, Tensor b_scales, Tensor? bias) -> ()",
+          _block_scaled_mm_impl, lambda out, a, b, a_scales, b_scales, bias: None)
+_register("qk_norm_rope",
+          "(Tensor! q, Tensor! k, Tensor qkv, int num_heads_q, int num_heads_k, int head_dim, float epsilon, Tensor q_weight, "
+          "Tensor k_weight, Tensor cos_sin_cache, Tensor positions, bool is_neox=True) -> ()",
+          _qk_norm_rope_impl, lambda q, k, qkv, num_heads_q, num_heads_k, head_dim, epsilon, q_weight, k_weight, cos_sin_cache,
+          positions, is_neox=True: None)
 
 _ops = getattr(torch.ops, _NS)
 
@@ -868,6 +1054,81 @@ def cutlass_scaled_mm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, s
     out = torch.empty((a.shape[0], b.shape[1]), dtype=out_dtype, device=a.device)
     _ops.cutlass_scaled_mm(out, a, b, scale_a, scale_b, bias)
     return out.view(*target_shape)
+
+
+def _group_scales(rows: int, columns: int, device: torch.device) -> torch.Tensor:
+    """[rows, groups], a group's scales of all rows next to each other: how ``block_scaled_mm`` reads them best."""
+    return torch.empty((-(-columns // FP8_GROUP), rows), dtype=torch.float32, device=device).t()
+
+
+def scaled_fp8_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP,
+                           output: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantise ``input`` [..., columns] (float16, bfloat16, float32) to FP8 (e4m3fn) in groups of 128 consecutive values of a row, the last
+    of which may be shorter: ``scale = max(max|x|, 1e-10) / 448``, ``code = fp8(x / scale)``.  Returns the codes (``output`` if given) and
+    the scales [rows, groups] (a transposed view: a group's scales are contiguous).  A group with a NaN is NaN; one with an
+    infinity has an infinite scale, NaN for the infinities and 0 for the rest."""
+    _check_group_size("scaled_fp8_group_quant", group_size)
+    _check(input.dim() > 0, "scaled_fp8_group_quant: input must have a last dimension")
+    if output is None:
+        output = torch.empty(input.shape, dtype=FP8_DTYPE, device=input.device)
+    columns = input.size(-1)
+    scale = _group_scales(input.numel() // columns if columns else 0, columns, input.device)
+    _ops.scaled_fp8_group_quant(output, input, scale)
+    return output, scale
+
+
+def silu_and_mul_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP) -> tuple[torch.Tensor, torch.Tensor]:
+    """``scaled_fp8_group_quant(silu(input[..., :d]) * input[..., d:])`` of [..., 2 d] in one pass, the product in fp32 until it is
+    quantised."""
+    _check_group_size("silu_and_mul_group_quant", group_size)
+    _check(input.dim() > 0 and input.size(-1) % 2 == 0, "silu_and_mul_group_quant: the last dimension of input must be even")
+    d = input.size(-1) // 2
+    output = torch.empty((*input.shape[:-1], d), dtype=FP8_DTYPE, device=input.device)
+    scale = _group_scales(input.numel() // (2 * d) if d else 0, d, input.device)
+    _ops.silu_and_mul_group_quant(output, input, scale)
+    return output, scale
+
+
+def rms_norm_group_quant(input: torch.Tensor, weight: torch.Tensor, epsilon: float, residual: torch.Tensor | None = None,
+                         residual_out: torch.Tensor | None = None,
+                         group_size: int = FP8_GROUP) -> tuple[torch.Tensor, torch.Tensor]:
+    """``scaled_fp8_group_quant(rms_norm(input) * weight)`` in one pass, everything in fp32 until it is quantised.  With a ``residual`` the
+    norm is that of ``input + residual``, and the sum, rounded to their type, goes to ``residual_out``, or to ``residual`` itself."""
+    _check_group_size("rms_norm_group_quant", group_size)
+    _check(input.dim() > 0, "rms_norm_group_quant: input must have a last dimension")
+    output = torch.empty(input.shape, dtype=FP8_DTYPE, device=input.device)
+    hidden = input.size(-1)
+    scale = _group_scales(input.numel() // hidden if hidden else 0, hidden, input.device)
+    _ops.rms_norm_group_quant(output, input, weight, scale, epsilon, residual, residual_out)
+    return output, scale
+
+
+def block_scaled_mm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, out_dtype: torch.dtype,
+                    bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``(scale_a * a) @ (scale_b * b) + bias`` with fp8 ``a`` [..., K] row-major and ``b`` [K, N] column-major, a scale for each 128 values of
+    K in a row of ``a`` (``scale_a`` [rows, ceil(K / 128)]) and one for each 128 x 128 block of ``b`` (``scale_b`` [ceil(K / 128), ceil(N / 128)]),
+    both with any strides.  K and N are multiples of 16.  Sums in fp32, one rounding."""
+    _check(a.dim() > 0 and b.dim() == 2, "block_scaled_mm: a must be [..., K], b [K, N]")
+    rows = a if a.dim() == 2 else a.reshape(-1, a.size(-1))
+    out = torch.empty((rows.size(0), b.size(1)), dtype=out_dtype, device=a.device)
+    _ops.block_scaled_mm(out, rows, b, scale_a, scale_b, bias)
+    return out if a.dim() == 2 else out.view(*a.shape[:-1], b.size(1))
+
+
+def qk_norm_rope(qkv: torch.Tensor, num_heads_q: int, num_heads_k: int, head_dim: int, epsilon: float, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.Tensor, is_neox: bool = True,
+                 q: torch.Tensor | None = None, k: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of each query and key head of a qkv projection's result ``qkv`` [tokens, queries | keys | ...] and the rotation by
+    ``positions`` (int64), in fp32 with one rounding.  ``cos_sin_cache`` [positions, rotary_dim] holds cosines, then sines, in float32 or qkv's
+    dtype; the first ``rotary_dim`` values of a head are rotated, in pairs ``(i, i + rotary_dim / 2)`` (``is_neox``) or ``(2 i, 2 i + 1)``.
+    Returns queries [tokens, num_heads_q, head_dim] and keys (``q`` and ``k`` if given); a token whose position is outside the
+    cache (padding) leaves its rows of them unwritten."""
+    if q is None:
+        q = torch.empty((qkv.size(0), num_heads_q, head_dim), dtype=qkv.dtype, device=qkv.device)
+    if k is None:
+        k = torch.empty((qkv.size(0), num_heads_k, head_dim), dtype=qkv.dtype, device=qkv.device)
+    _ops.qk_norm_rope(q, k, qkv, num_heads_q, num_heads_k, head_dim, epsilon, q_weight, k_weight, cos_sin_cache, positions, is_neox)
+    return q, k
 
 
 # ============================================================================ whole linear layers

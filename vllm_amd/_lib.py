@@ -61,6 +61,16 @@ _SIGNATURES = {
     "vaq_fp8_quant_scaled_mm_takes": (c_int, [c_int64, c_int64, c_int64, c_int]),
     "vaq_fp8_quant_scaled_mm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                         c_int64, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    "vaq_fp8_group_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                    c_void_p]),
+    "vaq_silu_and_mul_fp8_group_quant": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                                 c_int64, c_void_p]),
+    "vaq_rms_norm_fp8_group_quant": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, ctypes.c_float,
+                                             c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
+    "vaq_fp8_block_scaled_mm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    "vaq_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p]),
 }
 class VaqTuning(ctypes.Structure):
     """``VaqTuning`` of the header: kernel-variant overrides for ONE call (tests, benchmarks); all zero = automatic."""
@@ -72,7 +82,7 @@ class VaqTuning(ctypes.Structure):
 
 _TUNING_P = POINTER(VaqTuning)
 for _name in ("vaq_w4a16_gemm_workspace", "vaq_w4a16_gemm", "vaq_fp8_scaled_mm_workspace", "vaq_fp8_scaled_mm_ws",
-              "vaq_fp8_quant_per_token"):
+              "vaq_fp8_quant_per_token", "vaq_fp8_block_scaled_mm"):
     _res, _args = _SIGNATURES[_name]
     _SIGNATURES[_name + "_tuned"] = (_res, [*_args, _TUNING_P])
 

@@ -1,0 +1,162 @@
+// RMSNorm of every query and key head of a qkv projection's result and the rotation by the token's position, in one pass:
+//   y = x * rsqrt(mean of the head's squares + eps) * weight            (fp32)
+//   (u, v) -> (u cos - v sin, v cos + u sin)                            over pairs of the first `rotary` values, cos and sin from the position's row
+// and one rounding to the activations' type.  Pairs are (i, i + rotary / 2), or neighbours (2 i, 2 i + 1).
+//
+// Bound by memory: 2 bytes in and 2 out for each value, the row of cos and sin once a token.  A workgroup takes a token; a lane holds 8 consecutive values of a head
+// (16 bytes) and a head takes the next power of two of lanes, so that a wavefront has 512 values of several heads, and its sum of squares is a butterfly inside them.  cos, sin
+// and both weights stay in registers over the token's heads.  With pairs half the rotated width apart the partner's values come from the lane `rotary / 16` on.
+#include "vaq_common.h"
+
+namespace vaq {
+
+namespace {
+
+constexpr int QK_T = 256, QK_AHEAD = 4;      // threads; rounds of heads that are requested together
+
+struct QkArgs {
+  const uint16_t* qkv;
+  uint16_t *q, *k;
+  const uint16_t *q_weight, *k_weight;
+  const void* cache;
+  const int64_t* positions;
+  int64_t stride, cache_stride, cache_rows;
+  int heads_q, heads_k, head_dim, rotary, lanes_log2;      // lanes: of a head
+  float eps;
+};
+
+template <bool BF16>
+__device__ inline void unpack(v4u r, float (&f)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = F16Traits<BF16>::to_float((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+}
+
+template <bool BF16, bool CACHE32, bool HALVES>
+__global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
+  using T = F16Traits<BF16>;
+  const int64_t token = blockIdx.x, position = p.positions[token];
+  if (position < 0 || position >= p.cache_rows) return;      // not a token of a sequence: its rows stay as they are
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lanes = 1 << p.lanes_log2, per_wave = 64 >> p.lanes_log2;
+  const int e = (lane & (lanes - 1)) * 8;      // first of this lane's values in a head
+  const bool in_head = e < p.head_dim;
+  const int heads = p.heads_q + p.heads_k, rounds = (heads + per_wave - 1) / per_wave;
+  const uint16_t* const row = p.qkv + token * p.stride;
+
+  v4u x[QK_AHEAD];
+  auto head_of = [&](int round) { return round * per_wave + (lane >> p.lanes_log2); };
+  auto request = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < QK_AHEAD; ++i) {
+      const int h = head_of(first + i * (QK_T / 64));
+      x[i] = v4u{0u, 0u, 0u, 0u};
+      if (h < heads && in_head) x[i] = *reinterpret_cast<const v4u*>(row + (int64_t)h * p.head_dim + e);
+    }
+  };
+  int round = wave;
+  request(round);
+
+  // cos and sin of this lane's values; values that are not rotated have cos 1 and sin 0
+  float c[8], s[8], wq[8] = {}, wk[8] = {};
+  const int half = p.rotary / 2;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+    if (e + i < p.rotary) {
+      const int at = HALVES ? (e >= half ? e - half : e) + i : (e + i) / 2;
+      if constexpr (CACHE32) {
+        const float* const angle = (const float*)p.cache + position * p.cache_stride;
+        c[i] = angle[at];
+        s[i] = angle[half + at];
+      } else {
+        const uint16_t* const angle = (const uint16_t*)p.cache + position * p.cache_stride;
+        c[i] = T::to_float(angle[at]);
+        s[i] = T::to_float(angle[half + at]);
+      }
+      // the second of a pair has + sin, the first - sin
+      if (HALVES ? e < half : !(i & 1)) s[i] = -s[i];
+    }
+  }
+  if (in_head) {
+    unpack<BF16>(*reinterpret_cast<const v4u*>(p.q_weight + e), wq);
+    unpack<BF16>(*reinterpret_cast<const v4u*>(p.k_weight + e), wk);
+  }
+  // (HALVES: both halves of the rotated values are whole lanes)
+  const int partner = !HALVES || e >= p.rotary ? lane : e < half ? lane + half / 8 : lane - half / 8;
+
+  for (; round < rounds; round += QK_AHEAD * (QK_T / 64)) {
+    if (round != wave) request(round);
+#pragma unroll
+    for (int i = 0; i < QK_AHEAD; ++i) {
+      const int h = head_of(round + i * (QK_T / 64));
+      if (round + i * (QK_T / 64) >= rounds) break;      // (the same for the whole wavefront)
+      float y[8], ss = 0.f;
+      unpack<BF16>(x[i], y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+      for (int d = 1; d < lanes; d *= 2) ss += __shfl_xor(ss, d);
+      const float rms = rsqrtf(ss / (float)p.head_dim + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * rms * (h < p.heads_q ? wq[j] : wk[j]);
+      float z[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float other = HALVES ? __shfl(y[j], partner) : y[j ^ 1];
+        z[j] = y[j] * c[j];
+        if (e + j < p.rotary) z[j] += other * s[j];      // (a value that is not rotated stays what it is, whatever its neighbours are)
+      }
+      if (h < heads && in_head) {
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = (uint32_t)T::from_float(z[2 * j]) | (uint32_t)T::from_float(z[2 * j + 1]) << 16;
+        uint16_t* const to = h < p.heads_q ? p.q + (token * p.heads_q + h) * p.head_dim : p.k + (token * p.heads_k + h - p.heads_q) * p.head_dim;
+        *reinterpret_cast<v4u*>(to + e) = v4u{o[0], o[1], o[2], o[3]};
+      }
+    }
+  }
+}
+
+template <bool BF16>
+void launch(const QkArgs& a, bool cache32, bool halves, int64_t tokens, hipStream_t s) {
+  const dim3 grid((unsigned)tokens);
+  if (cache32 && halves) qk_norm_rope_kernel<BF16, true, true><<<grid, QK_T, 0, s>>>(a);
+  else if (cache32) qk_norm_rope_kernel<BF16, true, false><<<grid, QK_T, 0, s>>>(a);
+  else if (halves) qk_norm_rope_kernel<BF16, false, true><<<grid, QK_T, 0, s>>>(a);
+  else qk_norm_rope_kernel<BF16, false, false><<<grid, QK_T, 0, s>>>(a);
+}
+
+}  // namespace
+
+}  // namespace vaq
+
+using namespace vaq;
+
+extern "C" int vaq_qk_norm_rope(const void* qkv, int64_t qkv_row_stride, void* q_out, void* k_out, int64_t heads_q, int64_t heads_k, int64_t head_dim,
+                                float epsilon, const void* q_weight, const void* k_weight, const void* cos_sin, int cos_sin_dtype,
+                                int64_t cos_sin_row_stride, int64_t cos_sin_rows, int64_t rotary_dim, int interleaved, const int64_t* positions,
+                                int dtype, int64_t tokens, void* stream) {
+  VAQ_CHECK_ARG(dtype == VAQ_F16 || dtype == VAQ_BF16, "qk_norm_rope: dtype = %d", dtype);
+  VAQ_CHECK_ARG(cos_sin_dtype == VAQ_F32 || cos_sin_dtype == dtype, "qk_norm_rope: cos and sin are fp32 or of the type of qkv, not %d", cos_sin_dtype);
+  VAQ_CHECK_ARG(tokens >= 0 && tokens < (1ll << 31) && heads_q >= 0 && heads_k >= 0 && heads_q + heads_k > 0 && heads_q + heads_k <= 65536,
+                "qk_norm_rope: tokens = %lld, heads = %lld, %lld", (long long)tokens, (long long)heads_q, (long long)heads_k);
+  VAQ_CHECK_ARG(head_dim > 0 && rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 2 == 0, "qk_norm_rope: head_dim = %lld, rotary_dim = %lld",
+                (long long)head_dim, (long long)rotary_dim);
+  VAQ_CHECK_SUPPORTED(head_dim % 8 == 0 && head_dim <= 512, "qk_norm_rope: head_dim = %lld, a multiple of 8 up to 512 is built", (long long)head_dim);
+  VAQ_CHECK_SUPPORTED(interleaved || rotary_dim % 16 == 0, "qk_norm_rope: rotary_dim = %lld, pairs of halves need a multiple of 16", (long long)rotary_dim);
+  if (tokens == 0) return VAQ_OK;
+  VAQ_CHECK_ARG(qkv && (q_out || !heads_q) && (k_out || !heads_k) && q_weight && k_weight && positions && (cos_sin || !rotary_dim), "qk_norm_rope: null pointer");
+  VAQ_CHECK_ARG(tokens == 1 || qkv_row_stride >= (heads_q + heads_k) * head_dim, "qk_norm_rope: row stride %lld below the heads' values", (long long)qkv_row_stride);
+  VAQ_CHECK_ARG(cos_sin_rows >= 0 && (cos_sin_rows <= 1 || cos_sin_row_stride >= rotary_dim), "qk_norm_rope: cos_sin rows %lld, stride %lld",
+                (long long)cos_sin_rows, (long long)cos_sin_row_stride);
+  VAQ_CHECK_ARG((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight | (uintptr_t)k_weight) & 15) == 0 && (tokens == 1 || qkv_row_stride % 8 == 0),
+                "qk_norm_rope: rows and weights must be aligned to 16 bytes");
+  QkArgs a{(const uint16_t*)qkv, (uint16_t*)q_out, (uint16_t*)k_out, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos_sin, positions, qkv_row_stride,
+           cos_sin_row_stride, cos_sin_rows, (int)heads_q, (int)heads_k, (int)head_dim, (int)rotary_dim, 0, epsilon};
+  while ((8 << a.lanes_log2) < head_dim) ++a.lanes_log2;
+  if (dtype == VAQ_BF16) launch<true>(a, cos_sin_dtype == VAQ_F32, !interleaved, tokens, (hipStream_t)stream);
+  else launch<false>(a, cos_sin_dtype == VAQ_F32, !interleaved, tokens, (hipStream_t)stream);
+  VAQ_CHECK_LAUNCH("qk_norm_rope");
+  return VAQ_OK;
+}
