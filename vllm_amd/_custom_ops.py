@@ -1067,6 +1067,10 @@ def scaled_fp8_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP,
     of which may be shorter: ``scale = max(max|x|, 1e-10) / 448``, ``code = fp8(x / scale)``.  Returns the codes (``output`` if given) and
     the scales [rows, groups] (a transposed view: a group's scales are contiguous).  A group with a NaN is NaN; one with an
     infinity has an infinite scale, NaN for the infinities and 0 for the rest."""
+    if group_size == FP8_GROUP and not _tracing():
+        pair = _fast.group_quant(input, output)
+        if pair is not None:
+            return pair
     _check_group_size("scaled_fp8_group_quant", group_size)
     _check(input.dim() > 0, "scaled_fp8_group_quant: input must have a last dimension")
     if output is None:
@@ -1080,6 +1084,10 @@ def scaled_fp8_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP,
 def silu_and_mul_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP) -> tuple[torch.Tensor, torch.Tensor]:
     """``scaled_fp8_group_quant(silu(input[..., :d]) * input[..., d:])`` of [..., 2 d] in one pass, the product in fp32 until it is
     quantised."""
+    if group_size == FP8_GROUP and not _tracing():
+        pair = _fast.silu_group_quant(input)
+        if pair is not None:
+            return pair
     _check_group_size("silu_and_mul_group_quant", group_size)
     _check(input.dim() > 0 and input.size(-1) % 2 == 0, "silu_and_mul_group_quant: the last dimension of input must be even")
     d = input.size(-1) // 2
@@ -1094,6 +1102,10 @@ def rms_norm_group_quant(input: torch.Tensor, weight: torch.Tensor, epsilon: flo
                          group_size: int = FP8_GROUP) -> tuple[torch.Tensor, torch.Tensor]:
     """``scaled_fp8_group_quant(rms_norm(input) * weight)`` in one pass, everything in fp32 until it is quantised.  With a ``residual`` the
     norm is that of ``input + residual``, and the sum, rounded to their type, goes to ``residual_out``, or to ``residual`` itself."""
+    if group_size == FP8_GROUP and not _tracing():
+        pair = _fast.rms_norm_group_quant(input, weight, epsilon, residual, residual_out)
+        if pair is not None:
+            return pair
     _check_group_size("rms_norm_group_quant", group_size)
     _check(input.dim() > 0, "rms_norm_group_quant: input must have a last dimension")
     output = torch.empty(input.shape, dtype=FP8_DTYPE, device=input.device)
@@ -1108,6 +1120,10 @@ def block_scaled_mm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, sca
     """``(scale_a * a) @ (scale_b * b) + bias`` with fp8 ``a`` [..., K] row-major and ``b`` [K, N] column-major, a scale for each 128 values of
     K in a row of ``a`` (``scale_a`` [rows, ceil(K / 128)]) and one for each 128 x 128 block of ``b`` (``scale_b`` [ceil(K / 128), ceil(N / 128)]),
     both with any strides.  K and N are multiples of 16.  Sums in fp32, one rounding."""
+    if not _tracing():
+        out = _fast.block_mm(a, b, scale_a, scale_b, out_dtype, bias)
+        if out is not None:
+            return out
     _check(a.dim() > 0 and b.dim() == 2, "block_scaled_mm: a must be [..., K], b [K, N]")
     rows = a if a.dim() == 2 else a.reshape(-1, a.size(-1))
     out = torch.empty((rows.size(0), b.size(1)), dtype=out_dtype, device=a.device)
@@ -1123,6 +1139,10 @@ def qk_norm_rope(qkv: torch.Tensor, num_heads_q: int, num_heads_k: int, head_dim
     dtype; the first ``rotary_dim`` values of a head are rotated, in pairs ``(i, i + rotary_dim / 2)`` (``is_neox``) or ``(2 i, 2 i + 1)``.
     Returns queries [tokens, num_heads_q, head_dim] and keys (``q`` and ``k`` if given); a token whose position is outside the
     cache (padding) leaves its rows of them unwritten."""
+    if not _tracing():
+        pair = _fast.qk_norm_rope(qkv, num_heads_q, num_heads_k, head_dim, epsilon, q_weight, k_weight, cos_sin_cache, positions, is_neox, q, k)
+        if pair is not None:
+            return pair
     if q is None:
         q = torch.empty((qkv.size(0), num_heads_q, head_dim), dtype=qkv.dtype, device=qkv.device)
     if k is None:
@@ -1154,3 +1174,14 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
     """Quantise [..., K] activations (per token, or with the given per-tensor scale) and multiply: [..., N].  None where
     the two steps have to be taken one by one."""
     return None if _tracing() else _fast.fp8_linear(x, weight, weight_scale, input_scale, scale_ub, out_dtype, bias)
+
+
+def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, out_dtype: torch.dtype,
+                     bias: torch.Tensor | None) -> torch.Tensor:
+    """Quantise [..., K] activations in groups of 128 and multiply by a block-scaled weight [K, N]: [..., N]."""
+    if not _tracing():
+        out = _fast.block_fp8_linear(x, weight, weight_scale, out_dtype, bias)
+        if out is not None:
+            return out
+    codes, scale = scaled_fp8_group_quant(x)
+    return block_scaled_mm(codes, weight, scale, weight_scale, out_dtype, bias)

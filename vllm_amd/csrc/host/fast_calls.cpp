@@ -575,6 +575,221 @@ PyObject* py_silu_and_mul_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ FP8 in groups and blocks of 128
+
+// fp32 scales [rows, groups of `columns` values], a group's scales of all rows next to each other
+TensorBase group_scales(int64_t rows, int64_t columns, int device) {
+  const int64_t groups = (columns + 127) / 128;
+  TensorBase t = empty({rows * groups}, at::kFloat, device);
+  const int64_t size[2] = {rows, groups}, stride[2] = {1, rows};
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(size, stride);
+  return t;
+}
+
+// group_quant(input, output or None) -> (codes, scales) | None
+PyObject* py_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 2 || !plain_thread()) return decline();
+  Call call;
+  const TensorBase* x = call.tensor(v[0]);
+  const TensorBase* given = call.optional(v[1]);
+  if (!call.current()) return decline();
+  const int tag = dtype_tag(x->scalar_type());
+  int64_t rows = 0, ld = 0;
+  if (tag < 0 || x->dim() < 1 || x->size(-1) <= 0 || !as_rows(*x, x->size(-1), &rows, &ld) || rows <= 0) return decline();
+  const int64_t columns = x->size(-1);
+  if (given && (given->scalar_type() != at::kFloat8_e4m3fn || given->sizes() != x->sizes() || !given->is_contiguous())) return decline();
+  TensorBase out, scales;
+  int rc;
+  {
+    NoGil nogil;
+    out = given ? *given : empty(x->sizes(), at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, columns, call.device);
+    rc = vaq_fp8_group_quant(x->const_data_ptr(), tag, ld, (uint8_t*)out.mutable_data_ptr(), columns, (float*)scales.mutable_data_ptr(), 1, rows, rows,
+                             columns, stream_of(call.device));
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return Py_BuildValue("(NN)", given ? Py_NewRef(v[1]) : THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+// silu_group_quant(input) -> (codes, scales) | None
+PyObject* py_silu_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 1 || !plain_thread()) return decline();
+  Call call;
+  const TensorBase* x = call.tensor(v[0]);
+  if (!call.current()) return decline();
+  int64_t rows = 0, ld = 0;
+  if (!is16(x->scalar_type()) || x->dim() < 1 || x->size(-1) <= 0 || x->size(-1) % 2 != 0 || !as_rows(*x, x->size(-1), &rows, &ld) || rows <= 0)
+    return decline();
+  const int64_t d = x->size(-1) / 2;
+  TensorBase out, scales;
+  int rc;
+  {
+    NoGil nogil;
+    c10::SmallVector<int64_t, 6> size(x->sizes().begin(), x->sizes().end());
+    size.back() = d;
+    out = empty(size, at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, d, call.device);
+    rc = vaq_silu_and_mul_fp8_group_quant(x->const_data_ptr(), dtype_tag(x->scalar_type()), ld, (uint8_t*)out.mutable_data_ptr(), d,
+                                          (float*)scales.mutable_data_ptr(), 1, rows, rows, d, stream_of(call.device));
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_group_quant(input, weight, epsilon, residual or None, residual_out or None) -> (codes, scales) | None
+PyObject* py_rms_norm_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !plain_thread()) return decline();
+  Call call;
+  const TensorBase* x = call.tensor(v[0]);
+  const TensorBase* weight = call.tensor(v[1]);
+  const TensorBase* residual = call.optional(v[3]);
+  const TensorBase* place = call.optional(v[4]);
+  if (!call.current()) return decline();
+  const double eps = PyFloat_AsDouble(v[2]);
+  int64_t rows = 0, ld = 0;
+  if (PyErr_Occurred() || (place && !residual) || !norm_ok(*x, *weight, residual, &rows, &ld)) return decline();
+  if (!place) place = residual;
+  if (place && (place->scalar_type() != x->scalar_type() || !place->is_contiguous() || place->sizes() != x->sizes())) return decline();
+  TensorBase out, scales;
+  int rc;
+  {
+    NoGil nogil;
+    out = empty(x->sizes(), at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, x->size(-1), call.device);
+    rc = vaq_rms_norm_fp8_group_quant((uint8_t*)out.mutable_data_ptr(), (float*)scales.mutable_data_ptr(), 1, rows, x->const_data_ptr(), ld,
+                                      weight->const_data_ptr(), (float)eps, residual ? residual->const_data_ptr() : nullptr,
+                                      place ? place->mutable_data_ptr() : nullptr, dtype_tag(x->scalar_type()), rows, x->size(-1), stream_of(call.device));
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+// The weight [k, n], its scales [k / 128, n / 128] and the bias of a block-scaled GEMM.
+bool block_weight_ok(const TensorBase& b, const TensorBase& sb, const TensorBase* bias, int64_t k, ScalarType out_type) {
+  if (b.scalar_type() != at::kFloat8_e4m3fn || b.dim() != 2 || b.size(0) != k || b.stride(0) != 1 || b.stride(1) % 16 != 0) return false;
+  const int64_t n = b.size(1);
+  if (k <= 0 || n <= 0 || k % 16 != 0 || n % 16 != 0 || !is16(out_type) || !aligned16(b.const_data_ptr())) return false;
+  if (sb.scalar_type() != at::kFloat || sb.dim() != 2 || sb.size(0) != (k + 127) / 128 || sb.size(1) != (n + 127) / 128) return false;
+  return !bias || (bias->dim() == 1 && bias->numel() == n && bias->is_contiguous() && bias->scalar_type() == out_type);
+}
+// (without the lock)
+int block_mm(const void* a, int64_t lda, int64_t m, const float* sa, int64_t sa_row, int64_t sa_block, const TensorBase& b, const TensorBase& sb,
+             const TensorBase* bias, const TensorBase& out) {
+  return vaq_fp8_block_scaled_mm((const uint8_t*)a, lda, (const uint8_t*)b.const_data_ptr(), b.stride(1), sa, sa_row, sa_block,
+                                 (const float*)sb.const_data_ptr(), sb.stride(0), sb.stride(1), bias ? bias->const_data_ptr() : nullptr,
+                                 out.mutable_data_ptr(), b.size(1), dtype_tag(out.scalar_type()), m, b.size(1), b.size(0), stream_of(out.device().index()));
+}
+
+// block_mm(a, b, scale_a, scale_b, out_dtype, bias or None) -> Tensor [..., n] | None
+PyObject* py_block_mm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6 || !plain_thread() || !THPDtype_Check(v[4])) return decline();
+  Call call;
+  const TensorBase* a = call.tensor(v[0]);
+  const TensorBase* b = call.tensor(v[1]);
+  const TensorBase* sa = call.tensor(v[2]);
+  const TensorBase* sb = call.tensor(v[3]);
+  const TensorBase* bias = call.optional(v[5]);
+  if (!call.current()) return decline();
+  const ScalarType out_type = ((THPDtype*)v[4])->scalar_type;
+  if (b->dim() != 2 || a->scalar_type() != at::kFloat8_e4m3fn || !block_weight_ok(*b, *sb, bias, b->size(0), out_type)) return decline();
+  int64_t m = 0, lda = 0;
+  if (!as_rows(*a, b->size(0), &m, &lda) || m <= 0 || lda % 16 != 0 || lda < b->size(0) || !aligned16(a->const_data_ptr())) return decline();
+  if (sa->scalar_type() != at::kFloat || sa->dim() != 2 || sa->size(0) != m || sa->size(1) != sb->size(0)) return decline();
+  TensorBase out;
+  int rc;
+  {
+    NoGil nogil;
+    out = empty({m, b->size(1)}, out_type, call.device);
+    rc = block_mm(a->const_data_ptr(), lda, m, (const float*)sa->const_data_ptr(), sa->stride(0), sa->stride(1), *b, *sb, bias, out);
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return wrap_rows(*a, std::move(out), b->size(1));
+  END_HANDLE_TH_ERRORS
+}
+
+// block_fp8_linear(x, weight, weight_scale, out_dtype, bias or None) -> Tensor [..., n] | None
+// Activations quantised in groups, then the GEMM; the codes and their scales are one allocation that nobody else sees.
+PyObject* py_block_fp8_linear(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !plain_thread() || !THPDtype_Check(v[3])) return decline();
+  Call call;
+  const TensorBase* x = call.tensor(v[0]);
+  const TensorBase* b = call.tensor(v[1]);
+  const TensorBase* sb = call.tensor(v[2]);
+  const TensorBase* bias = call.optional(v[4]);
+  if (!call.current()) return decline();
+  const ScalarType out_type = ((THPDtype*)v[3])->scalar_type;
+  const int tag = dtype_tag(x->scalar_type());
+  if (tag < 0 || b->dim() != 2 || !block_weight_ok(*b, *sb, bias, b->size(0), out_type)) return decline();
+  const int64_t k = b->size(0), n = b->size(1), groups = sb->size(0);
+  int64_t m = 0, ldx = 0;
+  if (!as_rows(*x, k, &m, &ldx) || m <= 0) return decline();
+  TensorBase out;
+  int rc;
+  {
+    NoGil nogil;
+    out = empty({m, n}, out_type, call.device);
+    TensorBase held = empty({m * k + 4 * m * groups}, at::kByte, call.device);      // (m * k: a multiple of 16)
+    uint8_t* const codes = (uint8_t*)held.mutable_data_ptr();
+    float* const scales = (float*)(codes + m * k);
+    rc = vaq_fp8_group_quant(x->const_data_ptr(), tag, ldx, codes, k, scales, 1, m, m, k, stream_of(call.device));
+    if (rc == VAQ_OK) rc = block_mm(codes, k, m, scales, 1, m, *b, *sb, bias, out);
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return wrap_rows(*x, std::move(out), n);
+  END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rope(qkv, heads_q, heads_k, head_dim, epsilon, q_weight, k_weight, cos_sin, positions, is_neox, q or None, k or None) -> (q, k) | None
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 12 || !plain_thread()) return decline();
+  Call call;
+  const TensorBase* qkv = call.tensor(v[0]);
+  const TensorBase* wq = call.tensor(v[5]);
+  const TensorBase* wk = call.tensor(v[6]);
+  const TensorBase* cache = call.tensor(v[7]);
+  const TensorBase* positions = call.tensor(v[8]);
+  const TensorBase* q = call.optional(v[10]);
+  const TensorBase* k = call.optional(v[11]);
+  if (!call.current() || (v[9] != Py_True && v[9] != Py_False)) return decline();
+  const int64_t hq = PyLong_AsLongLong(v[1]), hk = PyLong_AsLongLong(v[2]), d = PyLong_AsLongLong(v[3]);
+  const double eps = PyFloat_AsDouble(v[4]);
+  if (PyErr_Occurred() || hq <= 0 || hk <= 0 || d <= 0 || hq > 65536 || hk > 65536 || d > 512) return decline();
+  const ScalarType type = qkv->scalar_type();
+  if (!is16(type) || qkv->dim() != 2 || qkv->stride(1) != 1 || qkv->size(1) < (hq + hk) * d || qkv->size(0) <= 0) return decline();
+  const int64_t tokens = qkv->size(0);
+  for (const TensorBase* w : {wq, wk})
+    if (w->scalar_type() != type || w->numel() != d || !w->is_contiguous()) return decline();
+  if (cache->dim() != 2 || (cache->scalar_type() != at::kFloat && cache->scalar_type() != type) || cache->stride(1) != 1) return decline();
+  if (positions->scalar_type() != at::kLong || positions->dim() != 1 || positions->numel() != tokens || !positions->is_contiguous()) return decline();
+  auto given_ok = [&](const TensorBase* t, int64_t heads) {
+    return !t || (t->scalar_type() == type && t->dim() == 3 && t->size(0) == tokens && t->size(1) == heads && t->size(2) == d && t->is_contiguous());
+  };
+  if (!given_ok(q, hq) || !given_ok(k, hk)) return decline();
+  TensorBase q_out, k_out;
+  int rc;
+  {
+    NoGil nogil;
+    q_out = q ? *q : empty({tokens, hq, d}, type, call.device);
+    k_out = k ? *k : empty({tokens, hk, d}, type, call.device);
+    rc = vaq_qk_norm_rope(qkv->const_data_ptr(), qkv->stride(0), q_out.mutable_data_ptr(), k_out.mutable_data_ptr(), hq, hk, d, (float)eps,
+                          wq->const_data_ptr(), wk->const_data_ptr(), cache->const_data_ptr(), dtype_tag(cache->scalar_type()), cache->stride(0),
+                          cache->size(0), cache->size(1), v[9] == Py_False, (const int64_t*)positions->const_data_ptr(), dtype_tag(type), tokens,
+                          stream_of(call.device));
+  }
+  if (rc != VAQ_OK) return raise_status(rc);
+  return Py_BuildValue("(NN)", q ? Py_NewRef(v[10]) : THPVariable_Wrap(std::move(q_out)), k ? Py_NewRef(v[11]) : THPVariable_Wrap(std::move(k_out)));
+  END_HANDLE_TH_ERRORS
+}
+
 // repack(codes, perm or None, k, n, bits, layout) -> Tensor | None; perm None: an AWQ checkpoint's tensor
 PyObject* py_repack(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -638,7 +853,8 @@ PyMethodDef g_methods[] = {
     {"setup", py_setup, METH_VARARGS, nullptr},
     {"tuned", py_tuned, METH_O, nullptr},
     FAST(w4_gemm), FAST(w4_linear), FAST(scaled_mm), FAST(fp8_linear), FAST(fp8_quant), FAST(rms_norm_dynamic_quant),
-    FAST(rms_norm_static_quant), FAST(silu_and_mul_quant), FAST(repack), {nullptr, nullptr, 0, nullptr}};
+    FAST(rms_norm_static_quant), FAST(silu_and_mul_quant), FAST(group_quant), FAST(silu_group_quant), FAST(rms_norm_group_quant),
+    FAST(block_mm), FAST(block_fp8_linear), FAST(qk_norm_rope), FAST(repack), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fast_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

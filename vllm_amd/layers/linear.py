@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from ..parameter import BasevLLMParameter, PerTensorScaleParameter, _ColumnvLLMParameter
+from ..parameter import BasevLLMParameter, BlockQuantScaleParameter, PerTensorScaleParameter, _ColumnvLLMParameter
 from .quantization.base_config import LinearMethodBase, QuantizationConfig
 from .quantization.utils.quant_utils import layer_tensor
 
@@ -76,6 +76,8 @@ class LinearBase(torch.nn.Module):
                     offset, size = self._part_offset_and_size(idx)
                     if param.packed_dim is not None and param.packed_dim == param.output_dim:
                         size, offset = param.adjust_shard_indexes_for_packing(size, offset)
+                    elif isinstance(param, BlockQuantScaleParameter):
+                        offset, size = param.block_range(offset, size)
                     self.weight_loader_v2(param, loaded_weight.narrow(param.output_dim, offset, size), idx)
             return
         offset, size = self._part_offset_and_size(loaded_shard_id)

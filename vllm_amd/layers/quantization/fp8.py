@@ -1,6 +1,6 @@
 """FP8 W8A8 quantization methods, same plugin surface as the reference's
-``vllm/model_executor/layers/quantization/fp8.py`` (Fp8Config :150-327, Fp8LinearMethod :330-684, non-block,
-non-Marlin branches) and ``ptpc_fp8.py`` (PTPCFp8LinearMethod :82-137: per-channel weights, per-token activations)."""
+``vllm/model_executor/layers/quantization/fp8.py`` (Fp8Config :150-327, Fp8LinearMethod :330-684, non-Marlin
+branches; weights with a scale for each block of 128 x 128) and ``ptpc_fp8.py`` (PTPCFp8LinearMethod :82-137: per-channel weights, per-token activations)."""
 from __future__ import annotations
 
 import os
@@ -10,12 +10,12 @@ import torch
 from torch.nn import Parameter
 
 from vllm_amd import _custom_ops as ops
-from vllm_amd.parameter import ModelWeightParameter, PerTensorScaleParameter
+from vllm_amd.parameter import BlockQuantScaleParameter, ModelWeightParameter, PerTensorScaleParameter
 from .base_config import LinearMethodBase, QuantizationConfig, QuantizeMethodBase
 from .input_quant_fp8 import GroupShape
 from .utils.marlin_utils_fp8 import apply_fp8_marlin_linear, prepare_fp8_layer_for_marlin
 from .utils.quant_utils import layer_tensor
-from .utils.w8a8_utils import Fp8LinearOp
+from .utils.w8a8_utils import Fp8LinearOp, W8A8BlockFp8LinearOp
 
 ACTIVATION_SCHEMES = ["static", "dynamic"]
 
@@ -30,8 +30,16 @@ class Fp8Config(QuantizationConfig):
         self.activation_scheme = activation_scheme
         self.ignored_layers = ignored_layers or []
         if weight_block_size is not None:
-            raise NotImplementedError("block-wise FP8 weights are not built for gfx950")
-        self.weight_block_size = None
+            if not is_checkpoint_fp8_serialized:
+                raise ValueError("block-wise FP8 weights come from a serialized FP8 checkpoint")
+            if len(weight_block_size) != 2:
+                raise ValueError(f"weight_block_size = {weight_block_size} must have two entries")
+            if activation_scheme != "dynamic":
+                raise ValueError(f"block-wise FP8 weights need dynamic activation scales, not {activation_scheme}")
+            if list(weight_block_size) != [ops.FP8_GROUP, ops.FP8_GROUP]:
+                raise NotImplementedError(f"weight_block_size = {list(weight_block_size)} is not built for gfx950 (only "
+                                          f"{[ops.FP8_GROUP, ops.FP8_GROUP]})")
+        self.weight_block_size = list(weight_block_size) if weight_block_size is not None else None
 
     @classmethod
     def get_name(cls) -> str:
@@ -68,19 +76,23 @@ class Fp8Config(QuantizationConfig):
 
 
 class Fp8LinearMethod(LinearMethodBase):
-    """FP8 linear: per-tensor weight scale, dynamic (per-token) or static (per-tensor) activation scale."""
+    """FP8 linear: per-tensor weight scale, dynamic (per-token) or static (per-tensor) activation scale; or a weight scale for each block of
+    128 x 128 (``weight_scale_inv`` of the checkpoint) and activation scales for groups of 128."""
 
     def __init__(self, quant_config: Fp8Config):
         self.quant_config = quant_config
         self.out_dtype = torch.get_default_dtype()
-        self.block_quant = False
+        self.block_quant = quant_config.weight_block_size is not None
         # Weight-only FP8 on the W4A16 GEMM: the reference takes this route on GPUs without FP8 matrix hardware or when
         # VLLM_TEST_FORCE_FP8_MARLIN is set (fp8.py:353-363).  gfx950 has FP8 MFMA: only when forced.
         self.use_marlin = os.environ.get("VLLM_TEST_FORCE_FP8_MARLIN", "0").lower() in ("1", "true")
+        if self.use_marlin and self.block_quant:
+            raise NotImplementedError("block-wise FP8 weights are not built for 16-bit activations")
         self.act_q_static = self.quant_config.activation_scheme == "static"
         # per-token activation scales whenever they are dynamic: the fused GEMM takes them at no extra cost
         self.act_q_group_shape = GroupShape.PER_TENSOR if self.act_q_static else GroupShape.PER_TOKEN
         self.fp8_linear = Fp8LinearOp(act_quant_static=self.act_q_static, act_quant_group_shape=self.act_q_group_shape)
+        self.block_linear = W8A8BlockFp8LinearOp() if self.block_quant else None
 
     def create_weights(self, layer: torch.nn.Module, input_size_per_partition: int, output_partition_sizes: list[int],
                        input_size: int, output_size: int, params_dtype: torch.dtype, **extra_weight_attrs):
@@ -89,13 +101,22 @@ class Fp8LinearMethod(LinearMethodBase):
         layer.input_size_per_partition = input_size_per_partition
         layer.output_size_per_partition = output_size_per_partition
         layer.orig_dtype = params_dtype
-        layer.weight_block_size = None
+        layer.weight_block_size = self.quant_config.weight_block_size
+        if self.block_quant:
+            self._check_blocks(input_size_per_partition, output_partition_sizes)
         weight_dtype = ops.FP8_DTYPE if self.quant_config.is_checkpoint_fp8_serialized else params_dtype
         loader = extra_weight_attrs.get("weight_loader")
         layer.register_parameter("weight", ModelWeightParameter(
             data=torch.empty(output_size_per_partition, input_size_per_partition, dtype=weight_dtype), input_dim=1,
             output_dim=0, weight_loader=loader))
-        if self.quant_config.is_checkpoint_fp8_serialized:
+        if self.block_quant:
+            block_n, block_k = layer.weight_block_size
+            layer.register_parameter("weight_scale_inv", BlockQuantScaleParameter(
+                data=torch.full((-(-output_size_per_partition // block_n), -(-input_size_per_partition // block_k)),
+                                torch.finfo(torch.float32).min, dtype=torch.float32), block_n=block_n, input_dim=1, output_dim=0,
+                weight_loader=loader))
+            layer.register_parameter("input_scale", None)
+        elif self.quant_config.is_checkpoint_fp8_serialized:
             # one scale per logical matrix of a fused layer, initialised to the most negative float so that the maximum
             # taken after loading ignores entries no checkpoint tensor filled (fp8.py:405-428)
             def per_part():
@@ -108,8 +129,20 @@ class Fp8LinearMethod(LinearMethodBase):
             else:
                 layer.register_parameter("input_scale", None)
 
+    def _check_blocks(self, input_size: int, output_sizes: list[int]) -> None:
+        block_n = self.quant_config.weight_block_size[0]
+        for size in output_sizes[:-1]:      # (the parts of a fused layer share no block; the last one may end inside its own)
+            if size % block_n != 0:
+                raise ValueError(f"Weight output_partition_size = {size} is not divisible by weight quantization block_n = {block_n}.")
+        if input_size % 16 != 0 or sum(output_sizes) % 16 != 0:
+            raise ValueError(f"block-wise FP8 layers need sizes that are multiples of 16, not {input_size} x {sum(output_sizes)}")
+
     def process_weights_after_loading(self, layer: torch.nn.Module) -> None:
         input_scale = None
+        if self.block_quant:
+            layer.weight = Parameter(layer.weight.data.t(), requires_grad=False)                        # [K, N] column-major view
+            layer.weight_scale_inv = Parameter(layer.weight_scale_inv.data.t(), requires_grad=False)    # [K / 128, N / 128]
+            return
         if not self.quant_config.is_checkpoint_fp8_serialized:
             # 16-bit checkpoint: quantise the weight per tensor on the device (fp8.py:497-500)
             qweight, weight_scale = ops.scaled_fp8_quant(layer.weight, scale=None)
@@ -153,6 +186,9 @@ class Fp8LinearMethod(LinearMethodBase):
             return apply_fp8_marlin_linear(input=x, weight=layer.weight, weight_scale=layer.weight_scale,
                                            workspace=layer.workspace, size_n=layer.output_size_per_partition,
                                            size_k=layer.input_size_per_partition, bias=bias)
+        if self.block_quant:
+            return self.block_linear.apply(x, layer_tensor(layer, "weight"), layer_tensor(layer, "weight_scale_inv"),
+                                           self.out_dtype if x.dtype not in (torch.float16, torch.bfloat16) else x.dtype, bias)
         return self.fp8_linear.apply(x, layer_tensor(layer, "weight"), layer_tensor(layer, "weight_scale"),
                                      self.out_dtype if x.dtype not in (torch.float16, torch.bfloat16) else x.dtype,
                                      layer_tensor(layer, "input_scale"), None, bias)

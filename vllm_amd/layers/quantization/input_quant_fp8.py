@@ -26,6 +26,7 @@ class GroupShape(NamedTuple):
 
 GroupShape.PER_TENSOR = GroupShape(-1, -1)
 GroupShape.PER_TOKEN = GroupShape(1, -1)
+GroupShape.PER_GROUP = GroupShape(1, ops.FP8_GROUP)      # 128 consecutive values of a token: the activations of block-scaled weights
 
 
 class QuantFP8(torch.nn.Module):
@@ -34,7 +35,7 @@ class QuantFP8(torch.nn.Module):
         self.static = static
         self.group_shape = group_shape
         self.num_token_padding = num_token_padding
-        assert group_shape in (GroupShape.PER_TOKEN, GroupShape.PER_TENSOR), "block-wise FP8 is not built"
+        assert group_shape in (GroupShape.PER_TOKEN, GroupShape.PER_TENSOR, GroupShape.PER_GROUP), f"{group_shape} is not built"
         assert not static or group_shape == GroupShape.PER_TENSOR, "Only per-tensor scales supported for static quantization."
         self.use_per_token_if_dynamic = group_shape == GroupShape.PER_TOKEN
 
@@ -43,6 +44,9 @@ class QuantFP8(torch.nn.Module):
         assert (scale is not None) == self.static
         assert scale_ub is None or (not self.static and self.group_shape == GroupShape.PER_TOKEN
                                     and scale_ub.numel() == 1)
+        if self.group_shape == GroupShape.PER_GROUP:
+            assert self.num_token_padding is None, "padding not supported with scales for groups"
+            return ops.scaled_fp8_group_quant(x)
         return ops.scaled_fp8_quant(x, scale, num_token_padding=self.num_token_padding, scale_ub=scale_ub,
                                     use_per_token_if_dynamic=self.use_per_token_if_dynamic)
 

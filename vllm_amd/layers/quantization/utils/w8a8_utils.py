@@ -61,3 +61,19 @@ class Fp8LinearOp:
                                                       per_tensor_activations)
         return w8a8_scaled_mm_func(qinput=qinput, weight=weight, out_dtype=out_dtype, scale_a=x_scale,
                                    scale_b=weight_scale, bias=bias, output_shape=output_shape)
+
+
+class W8A8BlockFp8LinearOp:
+    """FP8 linear op of block-scaled weights (reference: quantization/utils/fp8_utils.py): activations quantised in groups of 128, then the
+    product with a scale for each block of 128 x 128.  ``weight`` [K, N] column-major, ``weight_scale`` [K / 128, N / 128]."""
+
+    def __init__(self) -> None:
+        self.quant_fp8 = QuantFP8(static=False, group_shape=GroupShape.PER_GROUP)
+
+    def apply(self, input: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, out_dtype: torch.dtype | None = None,
+              bias: torch.Tensor | None = None) -> torch.Tensor:
+        quant = self.quant_fp8
+        if type(quant) is QuantFP8 and quant.runs_forward_only():
+            return ops.block_fp8_linear(input, weight, weight_scale, out_dtype or input.dtype, bias)
+        codes, scale = quant(input)
+        return ops.block_scaled_mm(codes, weight, scale, weight_scale, out_dtype or input.dtype, bias)

@@ -17,7 +17,7 @@ from typing import Callable
 import torch
 
 __all__ = ["BasevLLMParameter", "ModelWeightParameter", "RowvLLMParameter", "GroupQuantScaleParameter",
-           "ChannelQuantScaleParameter", "PerTensorScaleParameter", "PackedColumnParameter", "PackedvLLMParameter"]
+           "ChannelQuantScaleParameter", "PerTensorScaleParameter", "BlockQuantScaleParameter", "PackedColumnParameter", "PackedvLLMParameter"]
 
 _QKV_INDEX = {"q": 0, "k": 1, "v": 2}
 
@@ -141,6 +141,24 @@ class ModelWeightParameter(BasevLLMParameter):
 
 class GroupQuantScaleParameter(ModelWeightParameter):
     """Scales / zero points of group quantisation: [groups along the input dimension, output channels]."""
+
+
+class BlockQuantScaleParameter(ModelWeightParameter):
+    """Scales of a weight's blocks: [blocks along the output dimension, blocks along the input dimension], ``block_n`` output channels a
+    block.  The logical parts of a fused layer begin with a block (linear.py: the shard offsets of block scales)."""
+
+    def __init__(self, block_n: int, **kwargs):
+        super().__init__(**kwargs)
+        self._block_n = block_n
+
+    def block_range(self, shard_offset: int, shard_size: int) -> tuple[int, int]:
+        """(first block, blocks) of output channels [shard_offset, shard_offset + shard_size)."""
+        if shard_offset % self._block_n != 0:
+            raise ValueError(f"{type(self).__name__}: output channel {shard_offset} does not begin a block of {self._block_n}")
+        return shard_offset // self._block_n, -(-shard_size // self._block_n)
+
+    def _region(self, shard_offset: int, shard_size: int) -> torch.Tensor:
+        return super()._region(*self.block_range(shard_offset, shard_size))
 
 
 class ChannelQuantScaleParameter(_ColumnvLLMParameter):
