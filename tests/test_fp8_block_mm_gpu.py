@@ -9,7 +9,7 @@ from oracle import fp8_block as ob
 pytestmark = pytest.mark.gpu
 
 FP8 = torch.float8_e4m3fn
-SHAPES = 4      # tile shapes
+SHAPES = 5      # tile shapes
 ROWS = [(mb, j) for mb in (1, 2, 3, 4) for j in (1, 2, 4) if mb + 2 * j < 10]      # blocks of 16 rows, n-tiles
 
 

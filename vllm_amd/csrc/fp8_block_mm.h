@@ -39,7 +39,7 @@ constexpr uint32_t F8B_NOWHERE = 0x80000000u;      // an offset past every opera
 bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, hipStream_t s);
 bool fp8_block_rows_fits(int64_t K, int mb, int j);
 // tiles (fp8_block_tile_kernel.h)
-constexpr int F8B_SHAPES = 4;
+constexpr int F8B_SHAPES = 5;
 int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s);
 
 }  // namespace vaq

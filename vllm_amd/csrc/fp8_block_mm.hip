@@ -3,19 +3,27 @@
 
 namespace vaq {
 
+template <int BM, int BN, int WAVES, size_t LDS, typename Kernel>
+static int launch_tiles(const Fp8BlockParams& p, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s) {
+  const uint32_t tiles_m = ((uint32_t)p.M + BM - 1) / BM, tiles_n = ((uint32_t)p.N + BN - 1) / BN;
+  if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), LDS, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
+  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), LDS, s, p, tiles_m, tiles_n);
+  return VAQ_OK;
+}
 // tile shapes: rows, columns, wavefronts along both, stages of the ring
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST>
 static int launch_shape(const Fp8BlockParams& p, hipStream_t s) {
-  const uint32_t tiles_m = ((uint32_t)p.M + BM - 1) / BM, tiles_n = ((uint32_t)p.N + BN - 1) / BN;
-  constexpr size_t lds = (size_t)NST * (BM + BN) * F8B;
-  auto run = [&](auto kern, size_t (&reserved)[VAQ_MAX_DEVICES]) {
-    if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
-    hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES_M * WAVES_N * 64), lds, s, p, tiles_m, tiles_n);
-    return VAQ_OK;
-  };
   static size_t whole[VAQ_MAX_DEVICES], tail[VAQ_MAX_DEVICES];
-  return p.K % F8B != 0 ? run(fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail)
-                        : run(fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole);
+  constexpr size_t LDS = (size_t)NST * (BM + BN) * F8B;
+  return p.K % F8B != 0 ? launch_tiles<BM, BN, WAVES_M * WAVES_N, LDS>(p, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail, s)
+                        : launch_tiles<BM, BN, WAVES_M * WAVES_N, LDS>(p, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole, s);
+}
+template <bool BF16>
+static int launch_256(const Fp8BlockParams& p, hipStream_t s) {
+  static size_t whole[VAQ_MAX_DEVICES], tail[VAQ_MAX_DEVICES];
+  constexpr size_t LDS = 5 * 256 * F8B;
+  return p.K % F8B != 0 ? launch_tiles<256, 256, 8, LDS>(p, fp8_block_tile256_kernel<BF16, true>, tail, s)
+                        : launch_tiles<256, 256, 8, LDS>(p, fp8_block_tile256_kernel<BF16, false>, whole, s);
 }
 
 template <bool BF16>
@@ -24,7 +32,8 @@ static int launch_type(const Fp8BlockParams& p, int shape, hipStream_t s) {
     case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, s);
     case 1: return launch_shape<BF16, 64, 128, 2, 2, 4>(p, s);
     case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, s);
-    default: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, s);
+    case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, s);
+    default: return launch_256<BF16>(p, s);
   }
 }
 int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s) {
@@ -50,7 +59,7 @@ static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
       }
   }
   auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  plan.shape = tiles(128, 256) >= cus ? 3 : tiles(128, 128) >= cus / 2 ? 2 : tiles(64, 128) >= cus / 2 ? 1 : 0;
+  plan.shape = tiles(256, 256) >= cus ? 4 : tiles(128, 256) >= cus ? 3 : tiles(128, 128) >= cus / 2 ? 2 : tiles(64, 128) >= cus / 2 ? 1 : 0;
   return plan;
 }
 
