@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 FP8 = torch.float8_e4m3fn
 SHAPES = 5      # tile shapes
-ROWS = [(mb, j) for mb in (1, 2, 3, 4) for j in (1, 2, 4) if mb + 2 * j < 10]      # blocks of 16 rows, n-tiles
+ROWS = [(mb, j, ahead) for mb in (1, 2, 3, 4) for j in (1, 2, 4) for ahead in (1, 2) if mb + ahead * j < 10]      # blocks of 16 rows, n-tiles, steps ahead
 
 
 def make(m, k, n, dtype=torch.bfloat16, bias=False, seed=0):
@@ -58,12 +58,12 @@ def test_every_tile_shape(device, shape, m, k, n):
         check(call(c, device), c)
 
 
-@pytest.mark.parametrize("mb,j", ROWS)
+@pytest.mark.parametrize("mb,j,ahead", ROWS)
 @pytest.mark.parametrize("m,k,n", [(1, 16, 16), (15, 256, 48), (16, 1280, 144), (70, 2064, 208), (33, 3840, 64), (130, 4096, 80), (4, 9216, 128)])
-def test_every_plan_for_few_rows(device, mb, j, m, k, n):
+def test_every_plan_for_few_rows(device, mb, j, ahead, m, k, n):
     from vllm_amd import _tuning
     c = make(m, k, n, bias=m > 15)
-    with _tuning.override(fp8_path=1, exp=[0] * 11 + [mb << 4 | j]):
+    with _tuning.override(fp8_path=1, exp=[0] * 11 + [ahead << 8 | mb << 4 | j]):
         check(call(c, device), c)
 
 
@@ -71,8 +71,8 @@ def _variants():
     yield "automatic", {}
     for shape in range(SHAPES):
         yield f"tile shape {shape}", dict(fp8_path=2, fp8_tile_cfg=shape + 1)
-    for mb, j in ROWS:
-        yield f"rows {mb} x {j}", dict(fp8_path=1, exp=[0] * 11 + [mb << 4 | j])
+    for mb, j, ahead in ROWS:
+        yield f"rows {mb} x {j}, {ahead} ahead", dict(fp8_path=1, exp=[0] * 11 + [ahead << 8 | mb << 4 | j])
 
 
 def test_one_scale_each(device):

@@ -35,9 +35,9 @@ __device__ inline __amdgpu_buffer_rsrc_t f8b_rsrc(const void* base, uint32_t byt
 }
 constexpr uint32_t F8B_NOWHERE = 0x80000000u;      // an offset past every operand: arrives as zeros
 
-// few rows (fp8_block_rows_kernel.h): n-tiles and blocks of 16 rows of a workgroup.  false: not built, or no room in LDS
-bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, hipStream_t s);
-bool fp8_block_rows_fits(int64_t K, int mb, int j);
+// few rows (fp8_block_rows_kernel.h): blocks of 16 rows and n-tiles of a workgroup, steps that weights are ahead.  false: not built, or no room in LDS
+bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, int ahead, hipStream_t s);
+bool fp8_block_rows_fits(int64_t K, int mb, int j, int ahead);
 // tiles (fp8_block_tile_kernel.h)
 constexpr int F8B_SHAPES = 5;
 int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s);

@@ -42,7 +42,7 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStre
 
 // The kernel of a problem.
 struct F8bPlan {
-  int mb = 0, j = 0;      // few rows; mb = 0: tiles
+  int mb = 0, j = 0, ahead = 2;      // few rows; mb = 0: tiles
   int shape = 0;
 };
 static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
@@ -52,7 +52,7 @@ static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
     const int mb = (int)((M + 15) / 16);
     // as many n-tiles a workgroup as leave every compute unit one
     for (int j = 4; j >= 1; j /= 2)
-      if (fp8_block_rows_fits(K, mb, j) && (j == 1 || (N + 16 * j - 1) / (16 * j) >= cus)) {
+      if (fp8_block_rows_fits(K, mb, j, 2) && (j == 1 || (N + 16 * j - 1) / (16 * j) >= cus)) {
         plan.mb = mb;
         plan.j = j;
         return plan;
@@ -70,16 +70,17 @@ static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
   const bool rows_ok = (64 * p.sa_row + blocks * p.sa_block) * 4 < ((int64_t)1 << 31);
   F8bPlan plan = plan_of(p.M, p.N, p.K, rows_ok);
   if (t.fp8_path == 1) {
-    plan.mb = t.exp[11] >> 4;
+    plan.mb = t.exp[11] >> 4 & 15;
     plan.j = t.exp[11] & 15;
-    VAQ_CHECK_SUPPORTED(rows_ok && plan.mb > 0 && fp8_block_rows_fits(p.K, plan.mb, plan.j), "fp8_block_scaled_mm: no such plan for few rows");
+    plan.ahead = t.exp[11] >> 8;
+    VAQ_CHECK_SUPPORTED(rows_ok && plan.mb > 0 && fp8_block_rows_fits(p.K, plan.mb, plan.j, plan.ahead), "fp8_block_scaled_mm: no such plan for few rows");
   } else if (t.fp8_path == 2) {
     plan.mb = 0;
     plan.shape = t.fp8_tile_cfg - 1;
     VAQ_CHECK_SUPPORTED(plan.shape >= 0 && plan.shape < F8B_SHAPES, "fp8_block_scaled_mm: no such tile shape");
   }
   if (plan.mb > 0) {
-    if (!fp8_block_rows_launch(p, bf16, plan.mb, plan.j, s)) return VAQ_ERR_LAUNCH;
+    if (!fp8_block_rows_launch(p, bf16, plan.mb, plan.j, plan.ahead, s)) return VAQ_ERR_LAUNCH;
   } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, s); rc != VAQ_OK) {
     return rc;
   }

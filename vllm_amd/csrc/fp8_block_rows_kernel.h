@@ -2,7 +2,8 @@
 //
 //  * A wavefront multiplies one step of 256 bytes of K of MB * 16 rows with J neighbouring n-tiles of 16 columns; the wavefronts of a workgroup take a quarter of K
 //    each and share nothing until their sums meet in LDS: no barrier in the K loop, no hand-over between workgroups, no scratch.
-//  * Both operands come by direct-to-LDS loads of 4 rows x 256 contiguous bytes into a piece of LDS of the wavefront's own, weights two steps ahead, activations one.
+//  * Both operands come by direct-to-LDS loads of 4 rows x 256 contiguous bytes into a piece of LDS of the wavefront's own, activations one step ahead, weights
+//    AHEAD = one or two: two where the weights' way from memory counts, one where the LDS has room for larger results instead.
 //  * A wavefront's scales for all of its K range are requested ahead of the first operands, into LDS of its own: a request behind another is answered behind it,
 //    so that the first step's wait covers them and no step waits for scales.
 //  * Rows beyond MB * 16 are a further block of rows with workgroups of their own, side by side on the same XCD, so that they find the weights in its L2.
@@ -15,10 +16,10 @@ constexpr int F8BR_WAVES = 4, F8BR_STEP = 256;
 __host__ __device__ inline int f8br_steps(int K) { return ((K + F8BR_STEP - 1) / F8BR_STEP + F8BR_WAVES - 1) / F8BR_WAVES; }      // of a wavefront, at most
 __host__ __device__ inline int f8br_scales_a(int steps, int mb) { return (steps * 2 * mb * 16 + 63) / 64 * 64; }                  // floats; a load writes 64
 __host__ __device__ inline int f8br_scales_b(int steps) { return (steps * 2 + 63) / 64 * 64; }
-constexpr size_t f8br_operand_bytes(int mb, int j) { return (size_t)(mb + 2 * j) * 16 * F8BR_STEP; }                             // of a wavefront
-inline size_t f8br_lds_bytes(int64_t K, int mb, int j) {
+constexpr size_t f8br_operand_bytes(int mb, int j, int ahead) { return (size_t)(mb + ahead * j) * 16 * F8BR_STEP; }              // of a wavefront
+inline size_t f8br_lds_bytes(int64_t K, int mb, int j, int ahead) {
   const int steps = f8br_steps((int)K);
-  const size_t run = F8BR_WAVES * (f8br_operand_bytes(mb, j) + 4 * (size_t)(f8br_scales_a(steps, mb) + f8br_scales_b(steps)));
+  const size_t run = F8BR_WAVES * (f8br_operand_bytes(mb, j, ahead) + 4 * (size_t)(f8br_scales_a(steps, mb) + f8br_scales_b(steps)));
   const size_t sums = (size_t)F8BR_WAVES * j * mb * 1024;
   return run > sums ? run : sums;
 }
@@ -33,8 +34,8 @@ __host__ __device__ inline F8brUnit f8br_unit(uint32_t block, uint32_t ranges, u
 }
 
 // TAIL: K ends inside a step; of the last one each lane asks for the chunks before K, and the rest of both operands arrives as zeros.
-template <bool BF16, int MB, int J, bool TAIL>
-__global__ __launch_bounds__(F8BR_WAVES * 64, 2) void fp8_block_rows_kernel(const Fp8BlockParams p, const uint32_t ranges, const uint32_t row_blocks) {
+template <bool BF16, int MB, int J, int AHEAD, bool TAIL>
+__global__ __launch_bounds__(F8BR_WAVES * 64, MB * J >= 12 ? 1 : 2) void fp8_block_rows_kernel(const Fp8BlockParams p, const uint32_t ranges, const uint32_t row_blocks) {
   using T = F16Traits<BF16>;
   constexpr int NW = F8BR_WAVES, KT = F8BR_STEP, R = (J * MB + NW - 1) / NW, TB = 16 * KT, LI = TB / 1024, U = KT / F8B;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
@@ -47,8 +48,8 @@ __global__ __launch_bounds__(F8BR_WAVES * 64, 2) void fp8_block_rows_kernel(cons
 
   typedef __attribute__((address_space(3))) void* lds_ptr_t;
   const int scales_a = f8br_scales_a(per, MB), scales_b = f8br_scales_b(per);
-  uint8_t* const mine = lds8 + (size_t)w * (f8br_operand_bytes(MB, J) + 4 * (size_t)(scales_a + scales_b));
-  float* const sa_lds = reinterpret_cast<float*>(mine + f8br_operand_bytes(MB, J));
+  uint8_t* const mine = lds8 + (size_t)w * (f8br_operand_bytes(MB, J, AHEAD) + 4 * (size_t)(scales_a + scales_b));
+  float* const sa_lds = reinterpret_cast<float*>(mine + f8br_operand_bytes(MB, J, AHEAD));
   float* const sb_lds = sa_lds + scales_a;
 
   // scales: [block of K][row], then [block of K]; blocks past K and past this wavefront's arrive as zeros
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(F8BR_WAVES * 64, 2) void fp8_block_rows_kernel(cons
     __builtin_amdgcn_sched_barrier(0);
     if (refill_act) load_act(g + 1);
     __builtin_amdgcn_sched_barrier(0);
-    if (refill_w) load_w(s, g + 2);
+    if (refill_w) load_w(s, g + AHEAD);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -147,30 +148,43 @@ __global__ __launch_bounds__(F8BR_WAVES * 64, 2) void fp8_block_rows_kernel(cons
     }
   };
 
-  // W(0) A(0) W(1) | A(1) W(2) | A(2) W(3) | ..., `|` = a step: it starts when all but the weights requested behind its activations have been answered
-  auto wait = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J * LI) : "memory"); };
   int g = first;
   load_w(0, g);
   __builtin_amdgcn_sched_barrier(0);
   load_act(g);
   __builtin_amdgcn_sched_barrier(0);
-  load_w(1, g + 1);
-  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (AHEAD == 1) {
+    // W(0) A(0) | A(1) W(1) | A(2) W(2) | ..., `|` = a step: it starts when everything has been answered
 #pragma unroll 1
-  for (; g + 2 < last; g += 2) {
-    wait();
-    tile(0, g, true, true);
-    wait();
-    tile(1, g + 1, true, true);
-  }
-  if (g + 1 < last) {
-    wait();
-    tile(0, g, true, false);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    tile(1, g + 1, false, false);
-  } else if (g < last) {
-    wait();
-    tile(0, g, false, false);
+    for (; g + 1 < last; ++g) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      tile(0, g, true, true);
+    }
+    if (g < last) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      tile(0, g, false, false);
+    }
+  } else {
+    // W(0) A(0) W(1) | A(1) W(2) | A(2) W(3) | ..., it starts when all but the weights requested behind its activations have been answered
+    auto wait = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J * LI) : "memory"); };
+    load_w(1, g + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (; g + 2 < last; g += 2) {
+      wait();
+      tile(0, g, true, true);
+      wait();
+      tile(1, g + 1, true, true);
+    }
+    if (g + 1 < last) {
+      wait();
+      tile(0, g, true, false);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      tile(1, g + 1, false, false);
+    } else if (g < last) {
+      wait();
+      tile(0, g, false, false);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (what is requested past the end writes zeros into LDS)
 
@@ -195,6 +209,8 @@ __global__ __launch_bounds__(F8BR_WAVES * 64, 2) void fp8_block_rows_kernel(cons
   }
 }
 
-constexpr bool f8br_built(int mb, int j) { return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || j == 4) && F8BR_WAVES * f8br_operand_bytes(mb, j) < 160 * 1024; }
+constexpr bool f8br_built(int mb, int j, int ahead) {
+  return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || j == 4) && (ahead == 1 || ahead == 2) && F8BR_WAVES * f8br_operand_bytes(mb, j, ahead) < 160 * 1024;
+}
 
 }  // namespace vaq
