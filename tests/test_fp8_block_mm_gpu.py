@@ -54,8 +54,9 @@ def test_block_scaled_mm(device, m, k, n, dtype, bias):
 def test_every_tile_shape(device, shape, m, k, n):
     from vllm_amd import _tuning
     c = make(m, k, n, bias=m > 100)
-    with _tuning.override(fp8_path=2, fp8_tile_cfg=shape + 1):
-        check(call(c, device), c)
+    for rotate in (0, 1):
+        with _tuning.override(fp8_path=2, fp8_tile_cfg=shape + 1, exp=[0] * 12 + [rotate]):
+            check(call(c, device), c)
 
 
 @pytest.mark.parametrize("mb,j,ahead", ROWS)
@@ -71,6 +72,7 @@ def _variants():
     yield "automatic", {}
     for shape in range(SHAPES):
         yield f"tile shape {shape}", dict(fp8_path=2, fp8_tile_cfg=shape + 1)
+        yield f"tile shape {shape}, rotated", dict(fp8_path=2, fp8_tile_cfg=shape + 1, exp=[0] * 12 + [1])
     for mb, j, ahead in ROWS:
         yield f"rows {mb} x {j}, {ahead} ahead", dict(fp8_path=1, exp=[0] * 11 + [ahead << 8 | mb << 4 | j])
 

@@ -40,6 +40,6 @@ bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, in
 bool fp8_block_rows_fits(int64_t K, int mb, int j, int ahead);
 // tiles (fp8_block_tile_kernel.h)
 constexpr int F8B_SHAPES = 5;
-int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s);
+int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, bool rotate, hipStream_t s);
 
 }  // namespace vaq

@@ -3,47 +3,49 @@
 
 namespace vaq {
 
-template <int BM, int BN, int WAVES, size_t LDS, typename Kernel>
-static int launch_tiles(const Fp8BlockParams& p, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s) {
+template <int BM, int BN, int WAVES, typename Kernel, typename... More>
+static int launch_tiles(const Fp8BlockParams& p, size_t lds, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s, More... more) {
   const uint32_t tiles_m = ((uint32_t)p.M + BM - 1) / BM, tiles_n = ((uint32_t)p.N + BN - 1) / BN;
-  if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), LDS, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), LDS, s, p, tiles_m, tiles_n);
+  if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
+  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), lds, s, p, tiles_m, tiles_n, more...);
   return VAQ_OK;
 }
 // tile shapes: rows, columns, wavefronts along both, stages of the ring
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST>
-static int launch_shape(const Fp8BlockParams& p, hipStream_t s) {
+static int launch_shape(const Fp8BlockParams& p, bool rotate, hipStream_t s) {
   static size_t whole[VAQ_MAX_DEVICES], tail[VAQ_MAX_DEVICES];
-  constexpr size_t LDS = (size_t)NST * (BM + BN) * F8B;
-  return p.K % F8B != 0 ? launch_tiles<BM, BN, WAVES_M * WAVES_N, LDS>(p, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail, s)
-                        : launch_tiles<BM, BN, WAVES_M * WAVES_N, LDS>(p, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole, s);
+  const size_t lds = F8bRing<BM, BN, NST>::lds_bytes(p.K);
+  constexpr int W = WAVES_M * WAVES_N;
+  return p.K % F8B != 0 ? launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail, s, (uint32_t)rotate)
+                        : launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole, s, (uint32_t)rotate);
 }
 template <bool BF16>
 static int launch_256(const Fp8BlockParams& p, hipStream_t s) {
   static size_t whole[VAQ_MAX_DEVICES], tail[VAQ_MAX_DEVICES];
   constexpr size_t LDS = 5 * 256 * F8B;
-  return p.K % F8B != 0 ? launch_tiles<256, 256, 8, LDS>(p, fp8_block_tile256_kernel<BF16, true>, tail, s)
-                        : launch_tiles<256, 256, 8, LDS>(p, fp8_block_tile256_kernel<BF16, false>, whole, s);
+  return p.K % F8B != 0 ? launch_tiles<256, 256, 8>(p, LDS, fp8_block_tile256_kernel<BF16, true>, tail, s)
+                        : launch_tiles<256, 256, 8>(p, LDS, fp8_block_tile256_kernel<BF16, false>, whole, s);
 }
 
 template <bool BF16>
-static int launch_type(const Fp8BlockParams& p, int shape, hipStream_t s) {
+static int launch_type(const Fp8BlockParams& p, int shape, bool rotate, hipStream_t s) {
   switch (shape) {
-    case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, s);
-    case 1: return launch_shape<BF16, 64, 128, 2, 2, 4>(p, s);
-    case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, s);
-    case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, s);
+    case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, rotate, s);
+    case 1: return launch_shape<BF16, 64, 128, 2, 2, 6>(p, rotate, s);
+    case 2: return launch_shape<BF16, 128, 128, 2, 2, 4>(p, rotate, s);
+    case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, rotate, s);
     default: return launch_256<BF16>(p, s);
   }
 }
-int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s) {
-  return bf16 ? launch_type<true>(p, shape, s) : launch_type<false>(p, shape, s);
+int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, bool rotate, hipStream_t s) {
+  return bf16 ? launch_type<true>(p, shape, rotate, s) : launch_type<false>(p, shape, rotate, s);
 }
 
 // The kernel of a problem.
 struct F8bPlan {
   int mb = 0, j = 0, ahead = 2;      // few rows; mb = 0: tiles
   int shape = 0;
+  bool rotate = false;
 };
 static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
   F8bPlan plan;
@@ -77,11 +79,12 @@ static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
   } else if (t.fp8_path == 2) {
     plan.mb = 0;
     plan.shape = t.fp8_tile_cfg - 1;
+    plan.rotate = t.exp[12] != 0;
     VAQ_CHECK_SUPPORTED(plan.shape >= 0 && plan.shape < F8B_SHAPES, "fp8_block_scaled_mm: no such tile shape");
   }
   if (plan.mb > 0) {
     if (!fp8_block_rows_launch(p, bf16, plan.mb, plan.j, plan.ahead, s)) return VAQ_ERR_LAUNCH;
-  } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, s); rc != VAQ_OK) {
+  } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, plan.rotate, s); rc != VAQ_OK) {
     return rc;
   }
   VAQ_CHECK_LAUNCH("fp8_block_scaled_mm");
@@ -114,6 +117,7 @@ extern "C" int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, cons
   VAQ_CHECK_SUPPORTED(sa_row_stride <= (1 << 20) && sa_block_stride < limit && sb_k_stride < limit && (256 * sa_row_stride + blocks * sa_block_stride) * 4 < limit &&
                           blocks * sb_k_stride * 4 < limit,
                       "fp8_block_scaled_mm: scales of 256 rows or of a block of columns lie more than 2 GiB apart");
+  VAQ_CHECK_SUPPORTED(size_k <= 131072, "fp8_block_scaled_mm: K = %lld, at most 131072 is built", (long long)size_k);      // (the scales of a block of columns are in LDS)
   const int64_t most = (int64_t)1 << 31;
   VAQ_CHECK_SUPPORTED(((size_m + 15) / 16) * ((size_n + 15) / 16) < most, "fp8_block_scaled_mm: M = %lld, N = %lld", (long long)size_m, (long long)size_n);
   const Fp8BlockParams p{a, b, sa, sb, (const uint16_t*)bias, (uint16_t*)out, sa_row_stride, sb_n_stride, (uint32_t)sa_block_stride, (uint32_t)sb_k_stride,

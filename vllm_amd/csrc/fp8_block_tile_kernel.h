@@ -2,8 +2,6 @@
 //
 //  * BM x BN results a workgroup; a step is one block of K.  Both operands come by direct-to-LDS loads of whole 128-byte lines (8 rows an instruction) into a
 //    ring of NST stages; chunk c of a row lies at place c ^ (row / 2 & 7) of its 128 bytes, so that the 16 lanes that are served together hit all banks.
-//  * A wavefront holds its TM rows' scales of the step in registers, one load for 64 rows, multiplied by the weight's scale and spread over the four groups of
-//    16 lanes by swaps: no LDS for scales, and no place in the ring.
 //  * The products of 16 rows are issued ahead of the multiply-adds of the 16 rows before them, which then find their results ready: four multiply-adds go beside an
 //    instruction that keeps the matrix core for 32 cycles.
 #pragma once
@@ -27,19 +25,13 @@ __host__ __device__ inline F8bTile f8b_tile(uint32_t position, uint32_t tiles_m,
 // A wavefront's part of a tile: TM x TN results, from fragments of both operands in LDS rows of 128 bytes.
 template <bool BF16, int TM, int TN>
 struct F8bWave {
-  static constexpr int MT = TM / 16, NT = TN / 16, SL = TM <= 64 ? 1 : TM / 64;      // SL: loads of row scales
-  static_assert((TM == 32 || TM % 64 == 0) && TN <= F8B && F8B % TN == 0, "shape of a wavefront");
-  struct Scales {
-    float a[SL], b;
-  };
+  static constexpr int MT = TM / 16, NT = TN / 16;
+  static_assert(TN <= F8B && F8B % TN == 0, "the columns of a wavefront share their scale");
   v4f acc[MT][NT], part[NT];      // part, pend: the last products, which the next ones' multiply-adds add
   float scale[MT], pend;
   uint32_t lo, hi;                // a fragment: chunks q and q + 4 of 16 rows, 64 bytes apart one way or the other
-  __amdgpu_buffer_rsrc_t rsa, rsb;
-  uint32_t vsa[SL], sa_step, sb_step;
 
-  // rows from `row` on of the tile's first, `rows` of them in it; columns from n on
-  __device__ inline void start(const Fp8BlockParams& p, int m0, int row, int rows, int n, int n_tile) {
+  __device__ inline void start() {
     const int lane = threadIdx.x & 63, q = lane >> 4, r16 = lane & 15;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -50,41 +42,6 @@ struct F8bWave {
     pend = 0.f;
     lo = (uint32_t)(r16 * 128 + ((q ^ (r16 >> 1)) * 16));
     hi = lo ^ 64u;
-    rsa = f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, 0x7ffffffcu);
-    rsb = f8b_rsrc(p.sb + (int64_t)((n < p.N ? n : n_tile) / F8B) * p.sb_n, 0x7ffffffcu);
-#pragma unroll
-    for (int i = 0; i < SL; ++i) vsa[i] = (uint32_t)min(row + (TM == 32 ? lane & 31 : i * 64 + lane), rows - 1) * (uint32_t)p.sa_row * 4u;
-    sa_step = p.sa_block * 4u;
-    sb_step = p.sb_block * 4u;
-  }
-  // scales of block kb: of the rows (lane: row i * 64 + lane; 32 rows twice) and of the columns
-  __device__ inline Scales request_scales(uint32_t kb) const {
-    Scales s;
-#pragma unroll
-    for (int i = 0; i < SL; ++i) s.a[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, (int)vsa[i], (int)(kb * sa_step), 0));
-    s.b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsb, 0, (int)(kb * sb_step), 0));
-    return s;
-  }
-  // -> scale[i]: that of row i * 16 + r16, in all four groups of 16 lanes
-  __device__ inline void spread(const Scales& s) {
-    auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
-    auto f = [](auto x) { return __builtin_bit_cast(float, (uint32_t)x); };
-#pragma unroll
-    for (int i = 0; i < SL; ++i) {
-      const uint32_t v = u(s.a[i] * s.b);
-      const auto h = __builtin_amdgcn_permlane16_swap(v, v, false, false);      // groups of lanes 0 0 2 2, and 1 1 3 3
-      if constexpr (TM == 32) {
-        scale[0] = f(h[0]);
-        scale[1] = f(h[1]);
-      } else {
-        const auto e = __builtin_amdgcn_permlane32_swap((uint32_t)h[0], (uint32_t)h[0], false, false);
-        const auto o = __builtin_amdgcn_permlane32_swap((uint32_t)h[1], (uint32_t)h[1], false, false);
-        scale[4 * i] = f(e[0]);
-        scale[4 * i + 1] = f(o[0]);
-        scale[4 * i + 2] = f(e[1]);
-        scale[4 * i + 3] = f(o[1]);
-      }
-    }
   }
   __device__ inline v8i fragment(const uint8_t* rows) const {
     const v4i x = *reinterpret_cast<const v4i*>(rows + lo), y = *reinterpret_cast<const v4i*>(rows + hi);
@@ -136,17 +93,63 @@ struct F8bWave {
   }
 };
 
-// The compiler's schedule of a run of products: four multiply-adds, one product, `reads` LDS reads behind each row of them but the last.
-template <int ROWS, int NT, int READS>
+// The same with the rows' scales in registers: one load for 64 rows, multiplied by the columns' scale and spread over the four groups of 16 lanes by swaps.
+template <bool BF16, int TM, int TN>
+struct F8bWaveScales : F8bWave<BF16, TM, TN> {
+  using Base = F8bWave<BF16, TM, TN>;
+  using Base::scale;
+  static constexpr int SL = TM / 64;      // loads of row scales
+  static_assert(TM % 64 == 0, "scales are loaded for 64 rows");
+  struct Scales {
+    float a[SL], b;
+  };
+  __amdgpu_buffer_rsrc_t rsa, rsb;
+  uint32_t vsa[SL], sa_step, sb_step;
+  // rows from `row` on of the tile's, which begin at m0 and are `rows`; columns from n on
+  __device__ inline void start(const Fp8BlockParams& p, int m0, int row, int rows, int n, int n_tile) {
+    const int lane = threadIdx.x & 63;
+    Base::start();
+    rsa = f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, 0x7ffffffcu);
+    rsb = f8b_rsrc(p.sb + (int64_t)((n < p.N ? n : n_tile) / F8B) * p.sb_n, 0x7ffffffcu);
+#pragma unroll
+    for (int i = 0; i < SL; ++i) vsa[i] = (uint32_t)min(row + i * 64 + lane, rows - 1) * (uint32_t)p.sa_row * 4u;
+    sa_step = p.sa_block * 4u;
+    sb_step = p.sb_block * 4u;
+  }
+  // scales of block kb: of the rows (lane: row i * 64 + lane) and of the columns
+  __device__ inline Scales request_scales(uint32_t kb) const {
+    Scales s;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) s.a[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsa, (int)vsa[i], (int)(kb * sa_step), 0));
+    s.b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsb, 0, (int)(kb * sb_step), 0));
+    return s;
+  }
+  // -> scale[i]: that of row i * 16 + r16, in all four groups of 16 lanes
+  __device__ inline void spread(const Scales& s) {
+    auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
+    auto f = [](auto x) { return __builtin_bit_cast(float, (uint32_t)x); };
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const uint32_t v = u(s.a[i] * s.b);
+      const auto h = __builtin_amdgcn_permlane16_swap(v, v, false, false);      // groups of lanes 0 0 2 2, and 1 1 3 3
+      const auto e = __builtin_amdgcn_permlane32_swap((uint32_t)h[0], (uint32_t)h[0], false, false);
+      const auto o = __builtin_amdgcn_permlane32_swap((uint32_t)h[1], (uint32_t)h[1], false, false);
+      scale[4 * i] = f(e[0]);
+      scale[4 * i + 1] = f(o[0]);
+      scale[4 * i + 2] = f(e[1]);
+      scale[4 * i + 3] = f(o[1]);
+    }
+  }
+};
+
+// The compiler's schedule of N products: LDS reads, four multiply-adds, one product.
+template <int N, int READS>
 __device__ inline void f8b_order() {
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    }
-    if (READS && i + 1 < ROWS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  for (int i = 0; i < N; ++i) {
+    if (READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
   }
 }
 
@@ -192,67 +195,114 @@ struct F8bOperand {
   }
 };
 
+// BM x BN results through a ring of NST stages.  A step's fragments are in registers when it begins; its products run while the next step's fragments are read,
+// and its stage, which nobody needs any more, takes the operands NST steps on.  So NST - 1 steps are under way, and a step costs the longer of its LDS traffic and its products, and one
+// barrier.  The rows' scales travel with the operands (a load of four bytes a lane into the stage): loaded into registers a step ahead they would be answered behind
+// the operands of all steps under way, which the wait for them would then be a wait for.  The columns' scales of all of K are requested once, ahead of everything.
+template <int BM, int BN, int NST>
+struct F8bRing {
+  static constexpr int SCALES = BM * 128 + BN * 128, STAGE = SCALES + BM * 4;
+  static inline size_t lds_bytes(int64_t K) { return (size_t)NST * STAGE + (BN + F8B - 1) / F8B * 4 * (size_t)sb_floats((int)K); }
+  __host__ __device__ static inline int sb_floats(int K) { return ((K + F8B - 1) / F8B + 1 + 63) / 64 * 64; }      // of a block of columns: one past K, which is zero
+};
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST, bool TAIL>
-__global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
-  constexpr int NW = WAVES_M * WAVES_N, TM = BM / WAVES_M, TN = BN / WAVES_N, STAGE = (BM + BN) * 128;
+__global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n, const uint32_t rotate) {
+  constexpr int NW = WAVES_M * WAVES_N, TM = BM / WAVES_M, TN = BN / WAVES_N;
   using Wave = F8bWave<BF16, TM, TN>;
-  constexpr int MT = Wave::MT, NT = Wave::NT;
+  using Ring = F8bRing<BM, BN, NST>;
+  constexpr int MT = Wave::MT, NT = Wave::NT, NB = (BN + F8B - 1) / F8B;
+  static_assert(BM <= 64 * NW, "each wavefront asks for the scales of 64 rows");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WAVES_N, wn = wave % WAVES_N;
   const uint32_t position = f8b_position(blockIdx.x, tiles_m * tiles_n);
   if (position >= tiles_m * tiles_n) return;
   const F8bTile tile = f8b_tile(position, tiles_m, tiles_n, BM, BN);
-  const int m0 = tile.m0, n0 = tile.n0, rows = min(BM, p.M - m0);
+  const int m0 = tile.m0, n0 = tile.n0, rows = min(BM, p.M - m0), steps = (p.K + F8B - 1) / F8B;
+  // rotate: the tiles of a column start at different places of K and wrap around, so that the weights' rows are asked for at as many places at once
+  const int first = rotate ? (int)((uint32_t)(m0 / BM) * (uint32_t)steps / tiles_m) : 0;
 
   F8bOperand<BM, NW, TAIL> a;
   F8bOperand<BN, NW, TAIL> b;
   a.start(p.a, m0, rows, p.lda, p.K, wave);
   b.start(p.b, n0, min(BN, p.N - n0), p.ldb, p.K, wave);
   Wave w;
-  w.start(p, m0, wm * TM, rows, n0 + wn * TN, n0);
-  auto request = [&](int step, uint8_t* at) {
-    a.request((uint32_t)step * F8B, at);
-    b.request((uint32_t)step * F8B, at + BM * 128);
+  w.start();
+  typedef __attribute__((address_space(3))) void* lds_ptr_t;
+  const int sb_floats = Ring::sb_floats(p.K);
+  float* const sb_lds = reinterpret_cast<float*>(lds8 + NST * Ring::STAGE);      // [block of columns][block of K]
+  {
+    // (every wavefront asks for all of them: each then waits for its own requests only)
+    const int nb0 = n0 / F8B, nb_n = (p.N + F8B - 1) / F8B - nb0;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      for (int i = 0; i < sb_floats; i += 64)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sb + (int64_t)(nb0 + (nb < nb_n ? nb : 0)) * p.sb_n, 0x7ffffffcu), (lds_ptr_t)(sb_lds + nb * sb_floats + i), 4,
+                                                 (int)(i + lane < steps ? (uint32_t)(i + lane) * p.sb_block * 4u : F8B_NOWHERE), 0, 0, 0);
+  }
+  const __amdgpu_buffer_rsrc_t rsa = f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, 0x7ffffffcu);
+  const int sa_first = wave % (BM / 64) * 64;
+  const uint32_t vsa = (uint32_t)min(sa_first + lane, rows - 1) * (uint32_t)p.sa_row * 4u;
+  int kb_next = first, left = steps;      // the block that is requested next; how many are left
+  auto request = [&](uint8_t* at) {
+    const uint32_t k = left > 0 ? (uint32_t)kb_next * F8B : (uint32_t)p.K;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)(left > 0 ? vsa : F8B_NOWHERE),
+                                             left > 0 ? (int)((uint32_t)kb_next * p.sa_block * 4u) : 0, 0, 0);
+    a.request(k, at);
+    b.request(k, at + BM * 128);
+    kb_next = kb_next + 1 == steps ? 0 : kb_next + 1;
+    --left;
   };
-  auto compute = [&](const uint8_t* at, const typename Wave::Scales& s) {
-    v8i cols[NT], row[2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) cols[j] = w.fragment(at + BM * 128 + (wn * TN + j * 16) * 128);
-    row[0] = w.fragment(at + wm * TM * 128);
-    w.spread(s);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (i + 1 < MT) row[(i + 1) & 1] = w.fragment(at + (wm * TM + (i + 1) * 16) * 128);
-      w.multiply(i, cols, row[i & 1]);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * NT + 4, 0);
-    f8b_order<MT, NT, 2>();
+  struct Step {
+    v8i cols[NT], row[MT];
+    float sa[MT], sb;
   };
-
-  const int steps = (p.K + F8B - 1) / F8B;
-  constexpr int OPS = a.LD + b.LD, SCALES = Wave::SL + 1;      // requests of a step
-  // Behind a step's operands come those of the next NST - 2 steps and at least so many steps' scales: what may be under way when that step begins.
-  constexpr int BEHIND = (NST - 2) * OPS + (NST - 2 < 2 ? NST - 2 : 2) * SCALES;
-  static_assert(BEHIND <= 63, "wait counter range");
+  const uint8_t* const my_b = lds8 + BM * 128 + wn * TN * 128;
+  const uint8_t* const my_a = lds8 + wm * TM * 128;
+  const float* const my_sa = reinterpret_cast<const float*>(lds8 + Ring::SCALES) + wm * TM + (lane & 15);
+  const float* const my_sb = sb_lds + wn * TN / F8B * sb_floats;
+  int kb_read = first, to_read = steps;
+  auto read = [&](Step& f, int stage) {
+    const int at = stage * Ring::STAGE;
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) request(s, lds8 + s * STAGE);
-  typename Wave::Scales now = w.request_scales(0);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NST - 2) * OPS + SCALES) : "memory");
-  // Step s: its operands have landed for everybody and stage s - 1 has been read by everybody (the barrier ahead of it); the scales of step s + 1
-  // and the operands of step s + NST - 1 are requested.
+    for (int j = 0; j < NT; ++j) f.cols[j] = w.fragment(my_b + at + j * 2048);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) f.row[i] = w.fragment(my_a + at + i * 2048);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) f.sa[i] = my_sa[at / 4 + i * 16];
+    f.sb = my_sb[to_read > 0 ? kb_read : steps];
+    kb_read = kb_read + 1 == steps ? 0 : kb_read + 1;
+    --to_read;
+  };
+  // Behind a step's operands come those of the next NST - 2 steps.
+  constexpr int OPS = a.LD + b.LD + 1;
+  static_assert((NST - 1) * OPS <= 63, "wait counter range");
+#pragma unroll
+  for (int s = 0; s < NST; ++s) request(lds8 + s * Ring::STAGE);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NST - 1) * OPS) : "memory");
+  Step even, odd;
   int stage = 0;
+  auto on = [&](int q) { return q + 1 == NST ? 0 : q + 1; };
+  read(even, 0);
+  // One step: its fragments are here (lgkmcnt) and everybody's, so that its stage is free; the next one's operands have landed for everybody.
+  auto step = [&](Step& now, Step& next) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * OPS) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    request(lds8 + stage * Ring::STAGE);
+    stage = on(stage);
+    __builtin_amdgcn_sched_barrier(0);
+    read(next, stage);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) w.scale[i] = now.sa[i] * now.sb;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) w.multiply(i, now.cols, now.row[i]);
+    f8b_order<MT * NT, (2 * (NT + MT) + MT + 1 + MT * NT - 1) / (MT * NT)>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // (an odd number of steps ends with one of zeros)
 #pragma unroll 1
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_sched_barrier(0);
-    const typename Wave::Scales next = w.request_scales((uint32_t)min(s + 1, steps - 1));
-    __builtin_amdgcn_sched_barrier(0);
-    request(s + NST - 1, lds8 + (stage == 0 ? NST - 1 : stage - 1) * STAGE);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(lds8 + stage * STAGE, now);
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(BEHIND) : "memory");
-    now = next;
-    stage = stage + 1 == NST ? 0 : stage + 1;
+  for (int s = 0; s < steps; s += 2) {
+    step(even, odd);
+    step(odd, even);
   }
   w.store(p, m0 + wm * TM, n0 + wn * TN);
 }
@@ -265,7 +315,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(
 template <bool BF16, bool TAIL>
 __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
   constexpr int B = 256, NW = 8, TM = 128, TN = 64, PLACE = B * 128;
-  using Wave = F8bWave<BF16, TM, TN>;
+  using Wave = F8bWaveScales<BF16, TM, TN>;
   constexpr int NT = Wave::NT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
@@ -300,7 +350,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w.multiply(first + i, cols, row[i]);
-    f8b_order<4, NT, 0>();
+    f8b_order<4 * NT, 0>();
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
