@@ -31,8 +31,8 @@ template <bool BF16>
 static int launch_type(const Fp8BlockParams& p, int shape, bool rotate, hipStream_t s) {
   switch (shape) {
     case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, rotate, s);
-    case 1: return launch_shape<BF16, 64, 128, 2, 2, 6>(p, rotate, s);
-    case 2: return launch_shape<BF16, 128, 128, 2, 2, 4>(p, rotate, s);
+    case 1: return launch_shape<BF16, 64, 128, 2, 4, 6>(p, rotate, s);
+    case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, rotate, s);
     case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, rotate, s);
     default: return launch_256<BF16>(p, s);
   }

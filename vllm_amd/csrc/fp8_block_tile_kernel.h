@@ -195,6 +195,44 @@ struct F8bOperand {
   }
 };
 
+// The same with all of a lane's offsets in registers, so that a request is one instruction and its LDS address.
+template <int ROWS, int NW, bool TAIL>
+struct F8bOperandOffsets {
+  static constexpr int LD = ROWS / (8 * NW);
+  static_assert(LD >= 1, "fewer rows than the wavefronts ask for");
+  const uint8_t* base;
+  uint32_t v[LD], extent, lbyte, K;
+  int wave;
+  __device__ inline void start(const uint8_t* operand, int64_t first, int rows, uint32_t pitch, int K_, int wave_) {
+    const uint32_t lane = threadIdx.x & 63;
+    K = (uint32_t)K_;
+    wave = wave_;
+    base = operand + first * pitch;
+    extent = (uint32_t)(rows - 1) * pitch + K;
+    lbyte = ((lane & 7) ^ (lane >> 4)) * 16;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const uint32_t r0 = (uint32_t)(wave * LD + i) * 8, row = r0 + (lane >> 3);
+      v[i] = row < (uint32_t)rows ? row * pitch + (lbyte ^ (r0 & 8 ? 64u : 0u)) : F8B_NOWHERE;
+    }
+  }
+  // k = K: nothing
+  __device__ inline void request(uint32_t k, uint8_t* at) const {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const bool some = k < K;
+    const __amdgpu_buffer_rsrc_t r = f8b_rsrc(base, some ? extent : 0u);
+    const int so = some ? (int)k : 0;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const uint32_t r0 = (uint32_t)(wave * LD + i) * 8;
+      const bool odd = LD % 2 == 0 ? i & 1 : (r0 & 8) != 0;
+      uint32_t offset = v[i];
+      if constexpr (TAIL) offset = k + (lbyte ^ (odd ? 64u : 0u)) < K ? offset : F8B_NOWHERE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(at + r0 * 128), 16, (int)offset, so, 0, 0);
+    }
+  }
+};
+
 // BM x BN results through a ring of NST stages.  A step's fragments are in registers when it begins; its products run while the next step's fragments are read,
 // and its stage, which nobody needs any more, takes the operands NST steps on.  So NST - 1 steps are under way, and a step costs the longer of its LDS traffic and its products, and one
 // barrier.  The rows' scales travel with the operands (a load of four bytes a lane into the stage): loaded into registers a step ahead they would be answered behind
@@ -206,7 +244,7 @@ struct F8bRing {
   __host__ __device__ static inline int sb_floats(int K) { return ((K + F8B - 1) / F8B + 1 + 63) / 64 * 64; }      // of a block of columns: one past K, which is zero
 };
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST, bool TAIL>
-__global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n, const uint32_t rotate) {
+__global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n, const uint32_t rotate) {
   constexpr int NW = WAVES_M * WAVES_N, TM = BM / WAVES_M, TN = BN / WAVES_N;
   using Wave = F8bWave<BF16, TM, TN>;
   using Ring = F8bRing<BM, BN, NST>;
@@ -221,8 +259,8 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(
   // rotate: the tiles of a column start at different places of K and wrap around, so that the weights' rows are asked for at as many places at once
   const int first = rotate ? (int)((uint32_t)(m0 / BM) * (uint32_t)steps / tiles_m) : 0;
 
-  F8bOperand<BM, NW, TAIL> a;
-  F8bOperand<BN, NW, TAIL> b;
+  F8bOperandOffsets<BM, NW, TAIL> a;
+  F8bOperandOffsets<BN, NW, TAIL> b;
   a.start(p.a, m0, rows, p.lda, p.K, wave);
   b.start(p.b, n0, min(BN, p.N - n0), p.ldb, p.K, wave);
   Wave w;
@@ -239,17 +277,20 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(
         __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sb + (int64_t)(nb0 + (nb < nb_n ? nb : 0)) * p.sb_n, 0x7ffffffcu), (lds_ptr_t)(sb_lds + nb * sb_floats + i), 4,
                                                  (int)(i + lane < steps ? (uint32_t)(i + lane) * p.sb_block * 4u : F8B_NOWHERE), 0, 0, 0);
   }
-  const __amdgpu_buffer_rsrc_t rsa = f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, 0x7ffffffcu);
   const int sa_first = wave % (BM / 64) * 64;
-  const uint32_t vsa = (uint32_t)min(sa_first + lane, rows - 1) * (uint32_t)p.sa_row * 4u;
-  int kb_next = first, left = steps;      // the block that is requested next; how many are left
+  const uint32_t vsa = (uint32_t)min(sa_first + lane, rows - 1) * (uint32_t)p.sa_row * 4u, sa_step = p.sa_block * 4u;
+  uint32_t k_next = (uint32_t)first * F8B, sa_next = (uint32_t)first * sa_step;      // the block that is requested next
+  int left = steps;                                                                 // how many are left
   auto request = [&](uint8_t* at) {
-    const uint32_t k = left > 0 ? (uint32_t)kb_next * F8B : (uint32_t)p.K;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)(left > 0 ? vsa : F8B_NOWHERE),
-                                             left > 0 ? (int)((uint32_t)kb_next * p.sa_block * 4u) : 0, 0, 0);
+    const bool some = left > 0;
+    const uint32_t k = some ? k_next : (uint32_t)p.K;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, some ? 0x7ffffffcu : 0u), (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)vsa,
+                                             (int)(some ? sa_next : 0u), 0, 0);
     a.request(k, at);
     b.request(k, at + BM * 128);
-    kb_next = kb_next + 1 == steps ? 0 : kb_next + 1;
+    k_next += F8B;
+    sa_next += sa_step;
+    if (k_next >= (uint32_t)p.K) k_next = sa_next = 0;
     --left;
   };
   struct Step {
@@ -261,8 +302,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(
   const float* const my_sa = reinterpret_cast<const float*>(lds8 + Ring::SCALES) + wm * TM + (lane & 15);
   const float* const my_sb = sb_lds + wn * TN / F8B * sb_floats;
   int kb_read = first, to_read = steps;
-  auto read = [&](Step& f, int stage) {
-    const int at = stage * Ring::STAGE;
+  auto read = [&](Step& f, int at) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) f.cols[j] = w.fragment(my_b + at + j * 2048);
 #pragma unroll
@@ -280,15 +320,14 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64) void fp8_block_tile_kernel(
   for (int s = 0; s < NST; ++s) request(lds8 + s * Ring::STAGE);
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NST - 1) * OPS) : "memory");
   Step even, odd;
-  int stage = 0;
-  auto on = [&](int q) { return q + 1 == NST ? 0 : q + 1; };
+  int stage = 0;      // in bytes
   read(even, 0);
   // One step: its fragments are here (lgkmcnt) and everybody's, so that its stage is free; the next one's operands have landed for everybody.
   auto step = [&](Step& now, Step& next) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * OPS) : "memory");
     __builtin_amdgcn_sched_barrier(0);
-    request(lds8 + stage * Ring::STAGE);
-    stage = on(stage);
+    request(lds8 + stage);
+    stage = stage + Ring::STAGE == NST * Ring::STAGE ? 0 : stage + Ring::STAGE;
     __builtin_amdgcn_sched_barrier(0);
     read(next, stage);
 #pragma unroll
