@@ -142,14 +142,17 @@ struct F8bWaveScales : F8bWave<BF16, TM, TN> {
   }
 };
 
-// The compiler's schedule of N products: LDS reads, four multiply-adds, one product.
-template <int N, int READS>
+// The compiler's schedule of N products: LDS reads behind the first of them, a few at a time until there are READS, requests behind the others, and four multiply-adds ahead of each.
+template <int N, int READS, int REQUESTS>
 __device__ inline void f8b_order() {
+  constexpr int PER = READS == 0 ? 0 : (READS * 4 + 3 * N - 1) / (3 * N), WITH = READS == 0 ? 0 : (READS + PER - 1) / PER;      // (reads: three quarters of the products)
+  constexpr int LEFT = N > WITH ? N - WITH : 1, REQ = (REQUESTS + LEFT - 1) / LEFT;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
     __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (i < WITH) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    else if (REQUESTS) __builtin_amdgcn_sched_group_barrier(0x10, REQ, 0);
   }
 }
 
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   };
   const uint8_t* const my_b = lds8 + BM * 128 + wn * TN * 128;
   const uint8_t* const my_a = lds8 + wm * TM * 128;
-  const float* const my_sa = reinterpret_cast<const float*>(lds8 + Ring::SCALES) + wm * TM + (lane & 15);
+  const uint8_t* const my_sa = lds8 + Ring::SCALES + (wm * TM + (lane & 15)) * 4;
   const float* const my_sb = sb_lds + wn * TN / F8B * sb_floats;
   int kb_read = first, to_read = steps;
   auto read = [&](Step& f, int at) {
@@ -308,7 +311,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
 #pragma unroll
     for (int i = 0; i < MT; ++i) f.row[i] = w.fragment(my_a + at + i * 2048);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) f.sa[i] = my_sa[at / 4 + i * 16];
+    for (int i = 0; i < MT; ++i) f.sa[i] = *reinterpret_cast<const float*>(my_sa + at + i * 64);
     f.sb = my_sb[to_read > 0 ? kb_read : steps];
     kb_read = kb_read + 1 == steps ? 0 : kb_read + 1;
     --to_read;
@@ -326,15 +329,15 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   auto step = [&](Step& now, Step& next) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * OPS) : "memory");
     __builtin_amdgcn_sched_barrier(0);
-    request(lds8 + stage);
+    uint8_t* const free_stage = lds8 + stage;
     stage = stage + Ring::STAGE == NST * Ring::STAGE ? 0 : stage + Ring::STAGE;
-    __builtin_amdgcn_sched_barrier(0);
     read(next, stage);
 #pragma unroll
     for (int i = 0; i < MT; ++i) w.scale[i] = now.sa[i] * now.sb;
 #pragma unroll
     for (int i = 0; i < MT; ++i) w.multiply(i, now.cols, now.row[i]);
-    f8b_order<MT * NT, (2 * (NT + MT) + MT + 1 + MT * NT - 1) / (MT * NT)>();
+    request(free_stage);
+    f8b_order<MT * NT, 2 * (NT + MT) + MT + 1, OPS>();
     __builtin_amdgcn_sched_barrier(0);
   };
   // (an odd number of steps ends with one of zeros)
@@ -389,7 +392,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w.multiply(first + i, cols, row[i]);
-    f8b_order<4 * NT, 0>();
+    f8b_order<4 * NT, 0, 0>();
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
