@@ -113,11 +113,12 @@ def test_what_lies_around_the_operands(device, fill):
         sa, sw = torch.full((m + 64, kb + 9), float("nan"), device=device), torch.full((nb + 3, kb + 9), float("nan"), device=device)
         sa[:m, :kb], sw[:nb, :kb] = c["sa"].to(device), c["sw"].to(device)
         for name, fields in _variants():
-            held = torch.full((m + 300, n + 24), 3.0, dtype=torch.bfloat16, device=device)
-            with _tuning.override(**fields):
-                torch.ops.vllm_amd.block_scaled_mm(held[:m, 8:8 + n], a[:m, :k], w[:n, :k].t(), sa[:m, :kb], sw[:nb, :kb].t(), c["bias"].to(device))
-            check(held[:m, 8:8 + n], c, name)
-            assert bool((held[m:] == 3).all() and (held[:, :8] == 3).all() and (held[:, 8 + n:] == 3).all()), name
+            for first, pitch in ((8, n + 24), (4, n + 12)):      # rows aligned to 16 bytes and to 8
+                held = torch.full((m + 300, pitch), 3.0, dtype=torch.bfloat16, device=device)
+                with _tuning.override(**fields):
+                    torch.ops.vllm_amd.block_scaled_mm(held[:m, first:first + n], a[:m, :k], w[:n, :k].t(), sa[:m, :kb], sw[:nb, :kb].t(), c["bias"].to(device))
+                check(held[:m, first:first + n], c, name)
+                assert bool((held[m:] == 3).all() and (held[:, :first] == 3).all() and (held[:, first + n:] == 3).all()), name
 
 
 def test_operands_past_four_gigabytes(device):

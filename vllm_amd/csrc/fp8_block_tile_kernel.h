@@ -66,28 +66,54 @@ struct F8bWave {
     }
     if (i == MT - 1) pend = scale[MT - 1];
   }
-  // four neighbouring columns of a row a lane
-  __device__ inline void store(const Fp8BlockParams& p, int m, int n) {
+  // The products stand ahead of this, not behind the barrier that follows: the compiler may move what only a later phase uses.  (Nothing reads the registers here, so nothing
+  // waits for them.)
+  __device__ inline void hold() {
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(part[j]));
+#endif
+  }
+  // Results of the wavefront's part, which begins at (m, n).  They cross a piece of LDS of the wavefront's own (LDS_BYTES; everybody is done with the operands), 16 rows at a time, so
+  // that they leave as 16-byte stores, whole lines of 128 bytes.  As they lie in registers, a store of 8 bytes a lane touches 16 rows with 32 bytes each, and the
+  // requests of a device that finishes its tiles at the same time took 13 us.  Where the output is not aligned to 16 bytes they leave that way.
+  static constexpr int PITCH = TN * 2 + 16, LDS_BYTES = 16 * PITCH;
+  __device__ inline void store(const Fp8BlockParams& p, int m, int n, uint8_t* lds) {
     using T = F16Traits<BF16>;
     add(MT - 1, pend);
-    const int lane = threadIdx.x & 63;
-    m += lane & 15;
-    n += (lane >> 4) * 4;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r16 = lane & 15;
+    float bias[NT][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (n + j * 16 >= p.N) continue;
-      float bias[4] = {0.f, 0.f, 0.f, 0.f};
-      if (p.bias) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bias[e] = T::to_float(p.bias[n + j * 16 + e]);
+      for (int e = 0; e < 4; ++e) {
+        const int c = n + j * 16 + q * 4 + e;
+        bias[j][e] = p.bias && c < p.N ? T::to_float(p.bias[c]) : 0.f;
       }
+    const bool lines = ((uintptr_t)p.out & 15) == 0 && p.ldc % 8 == 0;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if (m + i * 16 >= p.M) continue;
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
         uint16_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = T::from_float(acc[i][j][e] + bias[e]);
-        *reinterpret_cast<v2u*>(p.out + (int64_t)(m + i * 16) * p.ldc + n + j * 16) = v2u{(uint32_t)o[0] | (uint32_t)o[1] << 16, (uint32_t)o[2] | (uint32_t)o[3] << 16};
+        for (int e = 0; e < 4; ++e) o[e] = T::from_float(acc[i][j][e] + bias[j][e]);
+        const v2u four{(uint32_t)o[0] | (uint32_t)o[1] << 16, (uint32_t)o[2] | (uint32_t)o[3] << 16};
+        if (lines) *reinterpret_cast<v2u*>(lds + r16 * PITCH + (j * 16 + q * 4) * 2) = four;
+        else if (m + i * 16 + r16 < p.M && n + j * 16 < p.N) *reinterpret_cast<v2u*>(p.out + (int64_t)(m + i * 16 + r16) * p.ldc + n + j * 16 + q * 4) = four;
+      }
+      if (lines) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();      // lanes exchange data through LDS; its operations run in program order
+        constexpr int CHUNKS = TN / 8;        // of 16 bytes in a row
+#pragma unroll
+        for (int c = 0; c < 16 * CHUNKS; c += 64) {
+          const int row = (c + lane) / CHUNKS, chunk = (c + lane) % CHUNKS;
+          const v4u eight = *reinterpret_cast<const v4u*>(lds + row * PITCH + chunk * 16);
+          if (m + i * 16 + row < p.M && n + chunk * 8 < p.N) *reinterpret_cast<v4u*>(p.out + (int64_t)(m + i * 16 + row) * p.ldc + n + chunk * 8) = eight;
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
       }
     }
   }
@@ -346,7 +372,9 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
     step(even, odd);
     step(odd, even);
   }
-  w.store(p, m0 + wm * TM, n0 + wn * TN);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (requests for nothing write zeros)
+  static_assert(NST * Ring::STAGE >= NW * Wave::LDS_BYTES, "room for the results");
+  w.store(p, m0 + wm * TM, n0 + wn * TN, lds8 + wave * Wave::LDS_BYTES);
 }
 
 // 256 x 256 results by eight wavefronts of 128 x 64 in alternating phases: of the two that share a SIMD one reads its fragments and requests operands while
@@ -392,6 +420,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w.multiply(first + i, cols, row[i]);
+    w.hold();
     f8b_order<4 * NT, 0, 0>();
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -420,7 +449,9 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     f8b_barrier_if(!late || s + 1 < steps);
     qb = qb >= 3 ? qb - 3 : qb + 2;
   }
-  w.store(p, m0 + wm * TM, n0 + wn * TN);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (requests for nothing write zeros)
+  static_assert(5 * PLACE >= NW * Wave::LDS_BYTES, "room for the results");
+  w.store(p, m0 + wm * TM, n0 + wn * TN, lds8 + wave * Wave::LDS_BYTES);
 }
 
 }  // namespace vaq
