@@ -171,7 +171,7 @@ struct F8bWaveScales : F8bWave<BF16, TM, TN> {
 // The compiler's schedule of N products: LDS reads behind the first of them, a few at a time until there are READS, requests behind the others, and four multiply-adds ahead of each.
 template <int N, int READS, int REQUESTS>
 __device__ inline void f8b_order() {
-  constexpr int PER = READS == 0 ? 0 : (READS * 4 + 3 * N - 1) / (3 * N), WITH = READS == 0 ? 0 : (READS + PER - 1) / PER;      // (reads: three quarters of the products)
+  constexpr int PER = READS == 0 ? 0 : READS == N ? 1 : (READS * 4 + 3 * N - 1) / (3 * N), WITH = READS == 0 ? 0 : (READS + PER - 1) / PER;      // (reads: three quarters of the products)
   constexpr int LEFT = N > WITH ? N - WITH : 1, REQ = (REQUESTS + LEFT - 1) / LEFT;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -380,8 +380,8 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
 // 256 x 256 results by eight wavefronts of 128 x 64 in alternating phases: of the two that share a SIMD one reads its fragments and requests operands while
 // the other one's products and multiply-adds run.  The LDS has five places for an operand of a step, which weights and activations take in turn, B(0) A(0) B(1) A(1) ...: a
 // step's weights are free behind its first phase, the activations behind its second, and each is at once replaced by what comes two and a half steps later.
-// A step of a wavefront is [read columns and rows 0 .. 63, request B(s + 2)] barrier [products] barrier [read rows 64 .. 127, request A(s + 2), wait for what step s + 1
-// reads] barrier [products] barrier; the late half of the workgroup passes one extra barrier first and skips its last one, so that every wavefront passes the same number.
+// A step of a wavefront is [read columns and rows 0 .. 31, request B(s + 2)] barrier [products of rows 0 .. 63, read rows 32 .. 95] barrier [read rows 96 .. 127, request A(s + 2),
+// wait for what step s + 1 reads] barrier [products of rows 64 .. 127] barrier; the late half of the workgroup passes one extra barrier first and skips its last one, so that every wavefront passes the same number.
 template <bool BF16, bool TAIL>
 __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
   constexpr int B = 256, NW = 8, TM = 128, TN = 64, PLACE = B * 128;
@@ -416,36 +416,47 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LD) : "memory");
   if (late) asm volatile("s_barrier" ::: "memory");
   v8i cols[NT], row[4];
-  auto products = [&](int first) {
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w.multiply(first + i, cols, row[i]);
-    w.hold();
-    f8b_order<4 * NT, 0, 0>();
-    __builtin_amdgcn_sched_barrier(0);
-  };
 #pragma unroll 1
   for (int s = 0; s < steps; ++s) {
     const uint8_t* const at_b = place(0) + wn * TN * 128;
     const uint8_t* const at_a = place(1) + wm * TM * 128;
 #pragma unroll
     for (int j = 0; j < NT; ++j) cols[j] = w.fragment(at_b + j * 2048);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) row[i] = w.fragment(at_a + i * 2048);
+    row[0] = w.fragment(at_a);
+    row[1] = w.fragment(at_a + 2048);
     w.spread(now);
     __builtin_amdgcn_sched_barrier(0);
     now = w.request_scales((uint32_t)min(s + 1, steps - 1));
     __builtin_amdgcn_sched_barrier(0);
     b.request((uint32_t)(s + 2) * F8B, place(4));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    products(0);
+    __builtin_amdgcn_sched_barrier(0);
+    row[2] = w.fragment(at_a + 2 * 2048);
+    row[3] = w.fragment(at_a + 3 * 2048);
+    w.multiply(0, cols, row[0]);
+    w.multiply(1, cols, row[1]);
+    row[0] = w.fragment(at_a + 4 * 2048);
+    row[1] = w.fragment(at_a + 5 * 2048);
+    w.multiply(2, cols, row[2]);
+    w.multiply(3, cols, row[3]);
+    w.hold();
+    f8b_order<NT, NT, 0>();
+    f8b_order<NT, 0, 0>();
+    f8b_order<NT, NT, 0>();
+    f8b_order<NT, 0, 0>();
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 4; ++i) row[i] = w.fragment(at_a + (4 + i) * 2048);
+    row[2] = w.fragment(at_a + 6 * 2048);
+    row[3] = w.fragment(at_a + 7 * 2048);
     __builtin_amdgcn_sched_barrier(0);
     a.request((uint32_t)(s + 2) * F8B, place(0));
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LD) : "memory");
-    products(4);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.multiply(4 + i, cols, row[i]);
+    w.hold();
+    f8b_order<4 * NT, 0, 0>();
+    __builtin_amdgcn_sched_barrier(0);
     f8b_barrier_if(!late || s + 1 < steps);
     qb = qb >= 3 ? qb - 3 : qb + 2;
   }
