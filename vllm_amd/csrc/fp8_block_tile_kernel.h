@@ -123,7 +123,6 @@ struct F8bWave {
 template <bool BF16, int TM, int TN>
 struct F8bWaveScales : F8bWave<BF16, TM, TN> {
   using Base = F8bWave<BF16, TM, TN>;
-  using Base::scale;
   static constexpr int SL = TM / 64;      // loads of row scales
   static_assert(TM % 64 == 0, "scales are loaded for 64 rows");
   struct Scales {
@@ -151,7 +150,7 @@ struct F8bWaveScales : F8bWave<BF16, TM, TN> {
     return s;
   }
   // -> scale[i]: that of row i * 16 + r16, in all four groups of 16 lanes
-  __device__ inline void spread(const Scales& s) {
+  __device__ inline void spread(const Scales& s, float (&scale)[TM / 16]) const {
     auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
     auto f = [](auto x) { return __builtin_bit_cast(float, (uint32_t)x); };
 #pragma unroll
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     const int q = qb + ahead;
     return lds8 + (q >= 5 ? q - 5 : q) * PLACE;
   };
-  typename Wave::Scales now = w.request_scales(0);
+  typename Wave::Scales first = w.request_scales(0), now = w.request_scales((uint32_t)min(1, steps - 1));
   b.request(0, place(0));
   a.request(0, place(1));
   b.request(F8B, place(2));
@@ -416,6 +415,8 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LD) : "memory");
   if (late) asm volatile("s_barrier" ::: "memory");
   v8i cols[NT], row[4];
+  float scale[Wave::MT];      // of the step to come
+  w.spread(first, scale);
 #pragma unroll 1
   for (int s = 0; s < steps; ++s) {
     const uint8_t* const at_b = place(0) + wn * TN * 128;
@@ -424,9 +425,8 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     for (int j = 0; j < NT; ++j) cols[j] = w.fragment(at_b + j * 2048);
     row[0] = w.fragment(at_a);
     row[1] = w.fragment(at_a + 2048);
-    w.spread(now);
-    __builtin_amdgcn_sched_barrier(0);
-    now = w.request_scales((uint32_t)min(s + 1, steps - 1));
+#pragma unroll
+    for (int i = 0; i < Wave::MT; ++i) w.scale[i] = scale[i];
     __builtin_amdgcn_sched_barrier(0);
     b.request((uint32_t)(s + 2) * F8B, place(4));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -449,11 +449,19 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     row[2] = w.fragment(at_a + 6 * 2048);
     row[3] = w.fragment(at_a + 7 * 2048);
     __builtin_amdgcn_sched_barrier(0);
+    const typename Wave::Scales next = w.request_scales((uint32_t)min(s + 2, steps - 1));
+    __builtin_amdgcn_sched_barrier(0);
     a.request((uint32_t)(s + 2) * F8B, place(0));
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LD) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LD + Wave::SL + 1) : "memory");
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w.multiply(4 + i, cols, row[i]);
+    w.spread(now, scale);      // (requested a step ago: ahead of everything that is still under way)
+    now = next;
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int i = 0; i < Wave::MT; ++i) asm volatile("" : "+v"(scale[i]));
+#endif
     w.hold();
     f8b_order<4 * NT, 0, 0>();
     __builtin_amdgcn_sched_barrier(0);
