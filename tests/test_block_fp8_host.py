@@ -194,7 +194,7 @@ def test_mm_plans_that_are_not_built():
     t = _lib.VaqTuning()
     t.fp8_path = 2
     refused("vaq_fp8_block_scaled_mm_tuned", [*base.values(), ctypes.byref(t)], NOT_BUILT, "tile shape")
-    t.fp8_path, t.exp[11] = 1, 2 << 8 | 4 << 4 | 4
+    t.fp8_path, t.exp[11] = 1, 4 << 12 | 2 << 8 | 4 << 4 | 4
     refused("vaq_fp8_block_scaled_mm_tuned", [*base.values(), ctypes.byref(t)], NOT_BUILT, "few rows")
 
 

@@ -9,8 +9,10 @@ from oracle import fp8_block as ob
 pytestmark = pytest.mark.gpu
 
 FP8 = torch.float8_e4m3fn
-SHAPES = 5      # tile shapes
-ROWS = [(mb, j, ahead) for mb in (1, 2, 3, 4) for j in (1, 2, 4) for ahead in (1, 2) if mb + ahead * j < 10]      # blocks of 16 rows, n-tiles, steps ahead
+SHAPES = 6      # tile shapes
+# blocks of 16 rows, n-tiles, steps ahead, wavefronts
+ROWS = [(mb, j, ahead, waves) for mb in (1, 2, 3, 4) for j in (1, 2, 4) for ahead in (1, 2) for waves in (4, 8)
+        if (mb + ahead * j) * waves < 40 and (waves == 4 or j == 1)]
 
 
 def make(m, k, n, dtype=torch.bfloat16, bias=False, seed=0):
@@ -59,12 +61,12 @@ def test_every_tile_shape(device, shape, m, k, n):
             check(call(c, device), c)
 
 
-@pytest.mark.parametrize("mb,j,ahead", ROWS)
+@pytest.mark.parametrize("mb,j,ahead,waves", ROWS)
 @pytest.mark.parametrize("m,k,n", [(1, 16, 16), (15, 256, 48), (16, 1280, 144), (70, 2064, 208), (33, 3840, 64), (130, 4096, 80), (4, 9216, 128)])
-def test_every_plan_for_few_rows(device, mb, j, ahead, m, k, n):
+def test_every_plan_for_few_rows(device, mb, j, ahead, waves, m, k, n):
     from vllm_amd import _tuning
     c = make(m, k, n, bias=m > 15)
-    with _tuning.override(fp8_path=1, exp=[0] * 11 + [ahead << 8 | mb << 4 | j]):
+    with _tuning.override(fp8_path=1, exp=[0] * 11 + [waves << 12 | ahead << 8 | mb << 4 | j]):
         check(call(c, device), c)
 
 
@@ -73,8 +75,8 @@ def _variants():
     for shape in range(SHAPES):
         yield f"tile shape {shape}", dict(fp8_path=2, fp8_tile_cfg=shape + 1)
         yield f"tile shape {shape}, rotated", dict(fp8_path=2, fp8_tile_cfg=shape + 1, exp=[0] * 12 + [1])
-    for mb, j, ahead in ROWS:
-        yield f"rows {mb} x {j}, {ahead} ahead", dict(fp8_path=1, exp=[0] * 11 + [ahead << 8 | mb << 4 | j])
+    for mb, j, ahead, waves in ROWS:
+        yield f"rows {mb} x {j}, {ahead} ahead, {waves} wavefronts", dict(fp8_path=1, exp=[0] * 11 + [waves << 12 | ahead << 8 | mb << 4 | j])
 
 
 def test_one_scale_each(device):

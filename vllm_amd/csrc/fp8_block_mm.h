@@ -35,11 +35,14 @@ __device__ inline __amdgpu_buffer_rsrc_t f8b_rsrc(const void* base, uint32_t byt
 }
 constexpr uint32_t F8B_NOWHERE = 0x80000000u;      // an offset past every operand: arrives as zeros
 
-// few rows (fp8_block_rows_kernel.h): blocks of 16 rows and n-tiles of a workgroup, steps that weights are ahead.  false: not built, or no room in LDS
-bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, int ahead, hipStream_t s);
-bool fp8_block_rows_fits(int64_t K, int mb, int j, int ahead);
+// few rows (fp8_block_rows_kernel.h): blocks of 16 rows and n-tiles of a workgroup, steps that weights are ahead, wavefronts.  false: not built, or no room in LDS
+struct F8bRows {
+  int mb = 0, j = 0, ahead = 0, waves = 0;
+};
+bool fp8_block_rows_fits(int64_t K, const F8bRows& r);
+bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, const F8bRows& r, hipStream_t s);
 // tiles (fp8_block_tile_kernel.h)
-constexpr int F8B_SHAPES = 5;
+constexpr int F8B_SHAPES = 6;
 int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, bool rotate, hipStream_t s);
 
 }  // namespace vaq

@@ -34,6 +34,7 @@ static int launch_type(const Fp8BlockParams& p, int shape, bool rotate, hipStrea
     case 1: return launch_shape<BF16, 64, 128, 2, 4, 6>(p, rotate, s);
     case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, rotate, s);
     case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, rotate, s);
+    case 4: return launch_shape<BF16, 256, 128, 4, 2, 3>(p, rotate, s);
     default: return launch_256<BF16>(p, s);
   }
 }
@@ -43,7 +44,7 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, bool ro
 
 // The kernel of a problem.
 struct F8bPlan {
-  int mb = 0, j = 0, ahead = 2;      // few rows; mb = 0: tiles
+  F8bRows rows;      // mb = 0: tiles
   int shape = 0;
   bool rotate = false;
 };
@@ -54,14 +55,13 @@ static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
     const int mb = (int)((M + 15) / 16);
     // as many n-tiles a workgroup as leave every compute unit one
     for (int j = 4; j >= 1; j /= 2)
-      if (fp8_block_rows_fits(K, mb, j, 2) && (j == 1 || (N + 16 * j - 1) / (16 * j) >= cus)) {
-        plan.mb = mb;
-        plan.j = j;
+      if (const F8bRows r{mb, j, 2, 4}; fp8_block_rows_fits(K, r) && (j == 1 || (N + 16 * j - 1) / (16 * j) >= cus)) {
+        plan.rows = r;
         return plan;
       }
   }
   auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  plan.shape = tiles(256, 256) >= cus ? 4 : tiles(128, 256) >= cus ? 3 : tiles(128, 128) >= cus / 2 ? 2 : tiles(64, 128) >= cus / 2 ? 1 : 0;
+  plan.shape = tiles(256, 256) >= cus ? 5 : tiles(128, 256) >= cus ? 3 : tiles(128, 128) >= cus / 2 ? 2 : tiles(64, 128) >= cus / 2 ? 1 : 0;
   return plan;
 }
 
@@ -72,18 +72,16 @@ static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
   const bool rows_ok = (64 * p.sa_row + blocks * p.sa_block) * 4 < ((int64_t)1 << 31);
   F8bPlan plan = plan_of(p.M, p.N, p.K, rows_ok);
   if (t.fp8_path == 1) {
-    plan.mb = t.exp[11] >> 4 & 15;
-    plan.j = t.exp[11] & 15;
-    plan.ahead = t.exp[11] >> 8;
-    VAQ_CHECK_SUPPORTED(rows_ok && plan.mb > 0 && fp8_block_rows_fits(p.K, plan.mb, plan.j, plan.ahead), "fp8_block_scaled_mm: no such plan for few rows");
+    plan.rows = F8bRows{t.exp[11] >> 4 & 15, t.exp[11] & 15, t.exp[11] >> 8 & 15, t.exp[11] >> 12};
+    VAQ_CHECK_SUPPORTED(rows_ok && fp8_block_rows_fits(p.K, plan.rows), "fp8_block_scaled_mm: no such plan for few rows");
   } else if (t.fp8_path == 2) {
-    plan.mb = 0;
+    plan.rows = F8bRows{};
     plan.shape = t.fp8_tile_cfg - 1;
     plan.rotate = t.exp[12] != 0;
     VAQ_CHECK_SUPPORTED(plan.shape >= 0 && plan.shape < F8B_SHAPES, "fp8_block_scaled_mm: no such tile shape");
   }
-  if (plan.mb > 0) {
-    if (!fp8_block_rows_launch(p, bf16, plan.mb, plan.j, plan.ahead, s)) return VAQ_ERR_LAUNCH;
+  if (plan.rows.mb > 0) {
+    if (!fp8_block_rows_launch(p, bf16, plan.rows, s)) return VAQ_ERR_LAUNCH;
   } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, plan.rotate, s); rc != VAQ_OK) {
     return rc;
   }

@@ -3,41 +3,42 @@
 
 namespace vaq {
 
-bool fp8_block_rows_fits(int64_t K, int mb, int j, int ahead) { return f8br_built(mb, j, ahead) && f8br_lds_bytes(K, mb, j, ahead) <= 160 * 1024; }
+bool fp8_block_rows_fits(int64_t K, const F8bRows& r) { return f8br_built(r.mb, r.j, r.ahead, r.waves) && f8br_lds_bytes(K, r.mb, r.j, r.ahead, r.waves) <= 160 * 1024; }
 
-template <bool BF16, int MB, int J, int AHEAD, bool TAIL>
+template <bool BF16, int MB, int J, int AHEAD, int NW, bool TAIL>
 static bool launch(const Fp8BlockParams& p, hipStream_t s) {
   const uint32_t ranges = ((uint32_t)p.N + 16 * J - 1) / (16 * J), row_blocks = ((uint32_t)p.M + MB * 16 - 1) / (MB * 16);
-  const size_t lds = f8br_lds_bytes(p.K, MB, J, AHEAD);
-  auto kern = fp8_block_rows_kernel<BF16, MB, J, AHEAD, TAIL>;
+  const size_t lds = f8br_lds_bytes(p.K, MB, J, AHEAD, NW);
+  auto kern = fp8_block_rows_kernel<BF16, MB, J, AHEAD, NW, TAIL>;
   static size_t reserved[VAQ_MAX_DEVICES];
   if (reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm") != VAQ_OK) return false;
-  hipLaunchKernelGGL(kern, dim3((ranges * row_blocks + 7) / 8 * 8), dim3(F8BR_WAVES * 64), lds, s, p, ranges, row_blocks);
+  hipLaunchKernelGGL(kern, dim3((ranges * row_blocks + 7) / 8 * 8), dim3(NW * 64), lds, s, p, ranges, row_blocks);
   return true;
 }
 
-template <int MB, int J, int AHEAD>
+template <int MB, int J, int AHEAD, int NW>
 static bool launch_plan(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
-  if constexpr (!f8br_built(MB, J, AHEAD)) {
+  if constexpr (!f8br_built(MB, J, AHEAD, NW)) {
     return false;
   } else {
     const bool tail = p.K % F8BR_STEP != 0;
-    if (bf16) return tail ? launch<true, MB, J, AHEAD, true>(p, s) : launch<true, MB, J, AHEAD, false>(p, s);
-    return tail ? launch<false, MB, J, AHEAD, true>(p, s) : launch<false, MB, J, AHEAD, false>(p, s);
+    if (bf16) return tail ? launch<true, MB, J, AHEAD, NW, true>(p, s) : launch<true, MB, J, AHEAD, NW, false>(p, s);
+    return tail ? launch<false, MB, J, AHEAD, NW, true>(p, s) : launch<false, MB, J, AHEAD, NW, false>(p, s);
   }
 }
-template <int MB, int AHEAD>
+template <int MB, int AHEAD, int NW>
 static bool launch_j(const Fp8BlockParams& p, bool bf16, int j, hipStream_t s) {
-  return j == 1 ? launch_plan<MB, 1, AHEAD>(p, bf16, s) : j == 2 ? launch_plan<MB, 2, AHEAD>(p, bf16, s) : launch_plan<MB, 4, AHEAD>(p, bf16, s);
+  return j == 1 ? launch_plan<MB, 1, AHEAD, NW>(p, bf16, s) : j == 2 ? launch_plan<MB, 2, AHEAD, NW>(p, bf16, s) : launch_plan<MB, 4, AHEAD, NW>(p, bf16, s);
 }
-template <int AHEAD>
+template <int AHEAD, int NW>
 static bool launch_mb(const Fp8BlockParams& p, bool bf16, int mb, int j, hipStream_t s) {
-  return mb == 1 ? launch_j<1, AHEAD>(p, bf16, j, s) : mb == 2 ? launch_j<2, AHEAD>(p, bf16, j, s) : mb == 3 ? launch_j<3, AHEAD>(p, bf16, j, s) : launch_j<4, AHEAD>(p, bf16, j, s);
+  return mb == 1 ? launch_j<1, AHEAD, NW>(p, bf16, j, s) : mb == 2 ? launch_j<2, AHEAD, NW>(p, bf16, j, s) : mb == 3 ? launch_j<3, AHEAD, NW>(p, bf16, j, s) : launch_j<4, AHEAD, NW>(p, bf16, j, s);
 }
 
-bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, int mb, int j, int ahead, hipStream_t s) {
-  if (!fp8_block_rows_fits(p.K, mb, j, ahead)) return false;
-  return ahead == 1 ? launch_mb<1>(p, bf16, mb, j, s) : launch_mb<2>(p, bf16, mb, j, s);
+bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, const F8bRows& r, hipStream_t s) {
+  if (!fp8_block_rows_fits(p.K, r)) return false;
+  if (r.waves == 8) return r.ahead == 1 ? launch_mb<1, 8>(p, bf16, r.mb, r.j, s) : launch_mb<2, 8>(p, bf16, r.mb, r.j, s);
+  return r.ahead == 1 ? launch_mb<1, 4>(p, bf16, r.mb, r.j, s) : launch_mb<2, 4>(p, bf16, r.mb, r.j, s);
 }
 
 }  // namespace vaq

@@ -1,7 +1,7 @@
 // FP8 product with a scale for each block of 128 (fp8_block_mm.h): few rows, bound by the weights' way from memory.
 //
-//  * A wavefront multiplies one step of 256 bytes of K of MB * 16 rows with J neighbouring n-tiles of 16 columns; the wavefronts of a workgroup take a quarter of K
-//    each and share nothing until their sums meet in LDS: no barrier in the K loop, no hand-over between workgroups, no scratch.
+//  * A wavefront multiplies one step of 256 bytes of K of MB * 16 rows with J neighbouring n-tiles of 16 columns; the NW wavefronts of a workgroup take a range of
+//    K each and share nothing until their sums meet in LDS: no barrier in the K loop, no hand-over between workgroups, no scratch.
 //  * Both operands come by direct-to-LDS loads of 4 rows x 256 contiguous bytes into a piece of LDS of the wavefront's own, activations one step ahead, weights
 //    AHEAD = one or two: two where the weights' way from memory counts, one where the LDS has room for larger results instead.
 //  * A wavefront's scales for all of its K range are requested ahead of the first operands, into LDS of its own: a request behind another is answered behind it,
@@ -12,15 +12,15 @@
 
 namespace vaq {
 
-constexpr int F8BR_WAVES = 4, F8BR_STEP = 256;
-__host__ __device__ inline int f8br_steps(int K) { return ((K + F8BR_STEP - 1) / F8BR_STEP + F8BR_WAVES - 1) / F8BR_WAVES; }      // of a wavefront, at most
+constexpr int F8BR_STEP = 256;
+__host__ __device__ inline int f8br_steps(int K, int nw) { return ((K + F8BR_STEP - 1) / F8BR_STEP + nw - 1) / nw; }      // of a wavefront, at most
 __host__ __device__ inline int f8br_scales_a(int steps, int mb) { return (steps * 2 * mb * 16 + 63) / 64 * 64; }                  // floats; a load writes 64
 __host__ __device__ inline int f8br_scales_b(int steps) { return (steps * 2 + 63) / 64 * 64; }
 constexpr size_t f8br_operand_bytes(int mb, int j, int ahead) { return (size_t)(mb + ahead * j) * 16 * F8BR_STEP; }              // of a wavefront
-inline size_t f8br_lds_bytes(int64_t K, int mb, int j, int ahead) {
-  const int steps = f8br_steps((int)K);
-  const size_t run = F8BR_WAVES * (f8br_operand_bytes(mb, j, ahead) + 4 * (size_t)(f8br_scales_a(steps, mb) + f8br_scales_b(steps)));
-  const size_t sums = (size_t)F8BR_WAVES * j * mb * 1024;
+inline size_t f8br_lds_bytes(int64_t K, int mb, int j, int ahead, int nw) {
+  const int steps = f8br_steps((int)K, nw);
+  const size_t run = nw * (f8br_operand_bytes(mb, j, ahead) + 4 * (size_t)(f8br_scales_a(steps, mb) + f8br_scales_b(steps)));
+  const size_t sums = (size_t)nw * j * mb * 1024;
   return run > sums ? run : sums;
 }
 
@@ -34,17 +34,17 @@ __host__ __device__ inline F8brUnit f8br_unit(uint32_t block, uint32_t ranges, u
 }
 
 // TAIL: K ends inside a step; of the last one each lane asks for the chunks before K, and the rest of both operands arrives as zeros.
-template <bool BF16, int MB, int J, int AHEAD, bool TAIL>
-__global__ __launch_bounds__(F8BR_WAVES * 64, MB * J >= 12 ? 1 : 2) void fp8_block_rows_kernel(const Fp8BlockParams p, const uint32_t ranges, const uint32_t row_blocks) {
+template <bool BF16, int MB, int J, int AHEAD, int NW, bool TAIL>
+__global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_block_rows_kernel(const Fp8BlockParams p, const uint32_t ranges, const uint32_t row_blocks) {
   using T = F16Traits<BF16>;
-  constexpr int NW = F8BR_WAVES, KT = F8BR_STEP, R = (J * MB + NW - 1) / NW, TB = 16 * KT, LI = TB / 1024, U = KT / F8B;
+  constexpr int KT = F8BR_STEP, R = (J * MB + NW - 1) / NW, TB = 16 * KT, LI = TB / 1024, U = KT / F8B;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
   const F8brUnit unit = f8br_unit(blockIdx.x, ranges, row_blocks);
   if (unit.range >= ranges) return;
   const int n0 = (int)unit.range * J * 16, row0 = (int)unit.rows * MB * 16;
   const uint32_t rows = (uint32_t)min(MB * 16, p.M - row0), columns = (uint32_t)min(J * 16, p.N - n0);
-  const int all = (p.K + KT - 1) / KT, per = f8br_steps(p.K), first = w * per, last = min(first + per, all);      // this wavefront's steps
+  const int all = (p.K + KT - 1) / KT, per = f8br_steps(p.K, NW), first = w * per, last = min(first + per, all);      // this wavefront's steps
 
   typedef __attribute__((address_space(3))) void* lds_ptr_t;
   const int scales_a = f8br_scales_a(per, MB), scales_b = f8br_scales_b(per);
@@ -209,8 +209,9 @@ __global__ __launch_bounds__(F8BR_WAVES * 64, MB * J >= 12 ? 1 : 2) void fp8_blo
   }
 }
 
-constexpr bool f8br_built(int mb, int j, int ahead) {
-  return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || j == 4) && (ahead == 1 || ahead == 2) && F8BR_WAVES * f8br_operand_bytes(mb, j, ahead) < 160 * 1024;
+constexpr bool f8br_built(int mb, int j, int ahead, int nw) {
+  return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || j == 4) && (ahead == 1 || ahead == 2) && (nw == 4 || (nw == 8 && j == 1)) &&
+         nw * f8br_operand_bytes(mb, j, ahead) < 160 * 1024;
 }
 
 }  // namespace vaq
