@@ -12,7 +12,7 @@ FP8 = torch.float8_e4m3fn
 SHAPES = 6      # tile shapes
 # blocks of 16 rows, n-tiles, steps ahead, wavefronts
 ROWS = [(mb, j, ahead, waves) for mb in (1, 2, 3, 4) for j in (1, 2, 4) for ahead in (1, 2) for waves in (4, 8)
-        if (mb + ahead * j) * waves < 40 and (waves == 4 or j == 1)]
+        if (mb + ahead * j) * waves < 40 and (waves == 4 or j == 1) and (j < 4 or ahead == 1)]
 
 
 def make(m, k, n, dtype=torch.bfloat16, bias=False, seed=0):
@@ -56,9 +56,8 @@ def test_block_scaled_mm(device, m, k, n, dtype, bias):
 def test_every_tile_shape(device, shape, m, k, n):
     from vllm_amd import _tuning
     c = make(m, k, n, bias=m > 100)
-    for rotate in (0, 1):
-        with _tuning.override(fp8_path=2, fp8_tile_cfg=shape + 1, exp=[0] * 12 + [rotate]):
-            check(call(c, device), c)
+    with _tuning.override(fp8_path=2, fp8_tile_cfg=shape + 1):
+        check(call(c, device), c)
 
 
 @pytest.mark.parametrize("mb,j,ahead,waves", ROWS)
@@ -74,7 +73,6 @@ def _variants():
     yield "automatic", {}
     for shape in range(SHAPES):
         yield f"tile shape {shape}", dict(fp8_path=2, fp8_tile_cfg=shape + 1)
-        yield f"tile shape {shape}, rotated", dict(fp8_path=2, fp8_tile_cfg=shape + 1, exp=[0] * 12 + [1])
     for mb, j, ahead, waves in ROWS:
         yield f"rows {mb} x {j}, {ahead} ahead, {waves} wavefronts", dict(fp8_path=1, exp=[0] * 11 + [waves << 12 | ahead << 8 | mb << 4 | j])
 

@@ -3,21 +3,21 @@
 
 namespace vaq {
 
-template <int BM, int BN, int WAVES, typename Kernel, typename... More>
-static int launch_tiles(const Fp8BlockParams& p, size_t lds, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s, More... more) {
+template <int BM, int BN, int WAVES, typename Kernel>
+static int launch_tiles(const Fp8BlockParams& p, size_t lds, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s) {
   const uint32_t tiles_m = ((uint32_t)p.M + BM - 1) / BM, tiles_n = ((uint32_t)p.N + BN - 1) / BN;
   if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), lds, s, p, tiles_m, tiles_n, more...);
+  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), lds, s, p, tiles_m, tiles_n);
   return VAQ_OK;
 }
 // tile shapes: rows, columns, wavefronts along both, stages of the ring
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST>
-static int launch_shape(const Fp8BlockParams& p, bool rotate, hipStream_t s) {
+static int launch_shape(const Fp8BlockParams& p, hipStream_t s) {
   static size_t whole[VAQ_MAX_DEVICES], tail[VAQ_MAX_DEVICES];
   const size_t lds = F8bRing<BM, BN, NST>::lds_bytes(p.K);
   constexpr int W = WAVES_M * WAVES_N;
-  return p.K % F8B != 0 ? launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail, s, (uint32_t)rotate)
-                        : launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole, s, (uint32_t)rotate);
+  return p.K % F8B != 0 ? launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, true>, tail, s)
+                        : launch_tiles<BM, BN, W>(p, lds, fp8_block_tile_kernel<BF16, BM, BN, WAVES_M, WAVES_N, NST, false>, whole, s);
 }
 template <bool BF16>
 static int launch_256(const Fp8BlockParams& p, hipStream_t s) {
@@ -28,25 +28,24 @@ static int launch_256(const Fp8BlockParams& p, hipStream_t s) {
 }
 
 template <bool BF16>
-static int launch_type(const Fp8BlockParams& p, int shape, bool rotate, hipStream_t s) {
+static int launch_type(const Fp8BlockParams& p, int shape, hipStream_t s) {
   switch (shape) {
-    case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, rotate, s);
-    case 1: return launch_shape<BF16, 64, 128, 2, 4, 6>(p, rotate, s);
-    case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, rotate, s);
-    case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, rotate, s);
-    case 4: return launch_shape<BF16, 256, 128, 4, 2, 3>(p, rotate, s);
+    case 0: return launch_shape<BF16, 64, 64, 2, 2, 6>(p, s);
+    case 1: return launch_shape<BF16, 64, 128, 2, 4, 6>(p, s);
+    case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, s);
+    case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, s);
+    case 4: return launch_shape<BF16, 256, 128, 4, 2, 3>(p, s);
     default: return launch_256<BF16>(p, s);
   }
 }
-int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, bool rotate, hipStream_t s) {
-  return bf16 ? launch_type<true>(p, shape, rotate, s) : launch_type<false>(p, shape, rotate, s);
+int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s) {
+  return bf16 ? launch_type<true>(p, shape, s) : launch_type<false>(p, shape, s);
 }
 
 // The kernel of a problem.
 struct F8bPlan {
   F8bRows rows;      // mb = 0: tiles
   int shape = 0;
-  bool rotate = false;
 };
 static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
   F8bPlan plan;
@@ -77,12 +76,11 @@ static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
   } else if (t.fp8_path == 2) {
     plan.rows = F8bRows{};
     plan.shape = t.fp8_tile_cfg - 1;
-    plan.rotate = t.exp[12] != 0;
     VAQ_CHECK_SUPPORTED(plan.shape >= 0 && plan.shape < F8B_SHAPES, "fp8_block_scaled_mm: no such tile shape");
   }
   if (plan.rows.mb > 0) {
     if (!fp8_block_rows_launch(p, bf16, plan.rows, s)) return VAQ_ERR_LAUNCH;
-  } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, plan.rotate, s); rc != VAQ_OK) {
+  } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, s); rc != VAQ_OK) {
     return rc;
   }
   VAQ_CHECK_LAUNCH("fp8_block_scaled_mm");

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
 }
 
 constexpr bool f8br_built(int mb, int j, int ahead, int nw) {
-  return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || j == 4) && (ahead == 1 || ahead == 2) && (nw == 4 || (nw == 8 && j == 1)) &&
+  return mb >= 1 && mb <= 4 && (j == 1 || j == 2 || (j == 4 && ahead == 1)) && (ahead == 1 || ahead == 2) && (nw == 4 || (nw == 8 && j == 1)) &&
          nw * f8br_operand_bytes(mb, j, ahead) < 160 * 1024;
 }
 

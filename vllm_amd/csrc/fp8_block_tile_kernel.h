@@ -167,17 +167,16 @@ struct F8bWaveScales : F8bWave<BF16, TM, TN> {
   }
 };
 
-// The compiler's schedule of N products: LDS reads behind the first of them, a few at a time until there are READS, requests behind the others, and four multiply-adds ahead of each.
-template <int N, int READS, int REQUESTS>
+// The compiler's schedule of N products, each behind four multiply-adds: READS LDS reads, the same number beside each of the first WITH products, and requests beside the others.
+template <int N, int READS, int WITH, int REQUESTS>
 __device__ inline void f8b_order() {
-  constexpr int PER = READS == 0 ? 0 : READS == N ? 1 : (READS * 4 + 3 * N - 1) / (3 * N), WITH = READS == 0 ? 0 : (READS + PER - 1) / PER;      // (reads: three quarters of the products)
-  constexpr int LEFT = N > WITH ? N - WITH : 1, REQ = (REQUESTS + LEFT - 1) / LEFT;
+  constexpr int R = WITH ? (READS + WITH - 1) / (WITH ? WITH : 1) : 0, Q = N > WITH ? (REQUESTS + N - WITH - 1) / (N > WITH ? N - WITH : 1) : 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    if (i < WITH) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-    else if (REQUESTS) __builtin_amdgcn_sched_group_barrier(0x10, REQ, 0);
+    if (i < WITH) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    else if (REQUESTS) __builtin_amdgcn_sched_group_barrier(0x10, Q, 0);
   }
 }
 
@@ -272,7 +271,7 @@ struct F8bRing {
   __host__ __device__ static inline int sb_floats(int K) { return ((K + F8B - 1) / F8B + 1 + 63) / 64 * 64; }      // of a block of columns: one past K, which is zero
 };
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST, bool TAIL>
-__global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n, const uint32_t rotate) {
+__global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
   constexpr int NW = WAVES_M * WAVES_N, TM = BM / WAVES_M, TN = BN / WAVES_N;
   using Wave = F8bWave<BF16, TM, TN>;
   using Ring = F8bRing<BM, BN, NST>;
@@ -284,9 +283,6 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   if (position >= tiles_m * tiles_n) return;
   const F8bTile tile = f8b_tile(position, tiles_m, tiles_n, BM, BN);
   const int m0 = tile.m0, n0 = tile.n0, rows = min(BM, p.M - m0), steps = (p.K + F8B - 1) / F8B;
-  // rotate: the tiles of a column start at different places of K and wrap around, so that the weights' rows are asked for at as many places at once
-  const int first = rotate ? (int)((uint32_t)(m0 / BM) * (uint32_t)steps / tiles_m) : 0;
-
   F8bOperandOffsets<BM, NW, TAIL> a;
   F8bOperandOffsets<BN, NW, TAIL> b;
   a.start(p.a, m0, rows, p.lda, p.K, wave);
@@ -307,19 +303,15 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   }
   const int sa_first = wave % (BM / 64) * 64;
   const uint32_t vsa = (uint32_t)min(sa_first + lane, rows - 1) * (uint32_t)p.sa_row * 4u, sa_step = p.sa_block * 4u;
-  uint32_t k_next = (uint32_t)first * F8B, sa_next = (uint32_t)first * sa_step;      // the block that is requested next
-  int left = steps;                                                                 // how many are left
+  uint32_t k = 0, sa_next = 0;      // the block that is requested next; past K: nothing
   auto request = [&](uint8_t* at) {
-    const bool some = left > 0;
-    const uint32_t k = some ? k_next : (uint32_t)p.K;
+    const bool some = k < (uint32_t)p.K;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, some ? 0x7ffffffcu : 0u), (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)vsa,
                                              (int)(some ? sa_next : 0u), 0, 0);
     a.request(k, at);
     b.request(k, at + BM * 128);
-    k_next += F8B;
+    k += F8B;
     sa_next += sa_step;
-    if (k_next >= (uint32_t)p.K) k_next = sa_next = 0;
-    --left;
   };
   struct Step {
     v8i cols[NT], row[MT];
@@ -329,7 +321,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   const uint8_t* const my_a = lds8 + wm * TM * 128;
   const uint8_t* const my_sa = lds8 + Ring::SCALES + (wm * TM + (lane & 15)) * 4;
   const float* const my_sb = sb_lds + wn * TN / F8B * sb_floats;
-  int kb_read = first, to_read = steps;
+  int kb_read = 0;
   auto read = [&](Step& f, int at) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) f.cols[j] = w.fragment(my_b + at + j * 2048);
@@ -337,9 +329,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
     for (int i = 0; i < MT; ++i) f.row[i] = w.fragment(my_a + at + i * 2048);
 #pragma unroll
     for (int i = 0; i < MT; ++i) f.sa[i] = *reinterpret_cast<const float*>(my_sa + at + i * 64);
-    f.sb = my_sb[to_read > 0 ? kb_read : steps];
-    kb_read = kb_read + 1 == steps ? 0 : kb_read + 1;
-    --to_read;
+    f.sb = my_sb[min(kb_read++, steps)];      // (past K: zero)
   };
   // Behind a step's operands come those of the next NST - 2 steps.
   constexpr int OPS = a.LD + b.LD + 1;
@@ -362,7 +352,7 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
 #pragma unroll
     for (int i = 0; i < MT; ++i) w.multiply(i, now.cols, now.row[i]);
     request(free_stage);
-    f8b_order<MT * NT, 2 * (NT + MT) + MT + 1, OPS>();
+    f8b_order<MT * NT, 2 * (NT + MT) + MT + 1, MT * NT / 4, OPS>();      // (reads beside three quarters of the products: 128 x 256 tiles 3 % slower)
     __builtin_amdgcn_sched_barrier(0);
   };
   // (an odd number of steps ends with one of zeros)
@@ -431,6 +421,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     b.request((uint32_t)(s + 2) * F8B, place(4));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
     row[2] = w.fragment(at_a + 2 * 2048);
     row[3] = w.fragment(at_a + 3 * 2048);
     w.multiply(0, cols, row[0]);
@@ -440,11 +431,12 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     w.multiply(2, cols, row[2]);
     w.multiply(3, cols, row[3]);
     w.hold();
-    f8b_order<NT, NT, 0>();
-    f8b_order<NT, 0, 0>();
-    f8b_order<NT, NT, 0>();
-    f8b_order<NT, 0, 0>();
+    f8b_order<NT, NT, NT, 0>();
+    f8b_order<NT, 0, 0, 0>();
+    f8b_order<NT, NT, NT, 0>();
+    f8b_order<NT, 0, 0, 0>();
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     asm volatile("s_barrier" ::: "memory");
     row[2] = w.fragment(at_a + 6 * 2048);
     row[3] = w.fragment(at_a + 7 * 2048);
@@ -454,6 +446,7 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     a.request((uint32_t)(s + 2) * F8B, place(0));
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LD + Wave::SL + 1) : "memory");
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w.multiply(4 + i, cols, row[i]);
     w.spread(now, scale);      // (requested a step ago: ahead of everything that is still under way)
@@ -463,8 +456,9 @@ __global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockPa
     for (int i = 0; i < Wave::MT; ++i) asm volatile("" : "+v"(scale[i]));
 #endif
     w.hold();
-    f8b_order<4 * NT, 0, 0>();
+    f8b_order<4 * NT, 0, 0, 0>();
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     f8b_barrier_if(!late || s + 1 < steps);
     qb = qb >= 3 ? qb - 3 : qb + 2;
   }

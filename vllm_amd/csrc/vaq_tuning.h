@@ -72,8 +72,7 @@ int vaq_fp8_quant_per_token_tuned(const void* in, int in_dtype, int64_t in_row_s
                                   int64_t hidden, void* stream, const VaqTuning* tuning);
 
 /* (fp8_path 1: the kernel for few rows, exp[11] = n-tiles | blocks of 16 rows << 4 | steps that weights are ahead << 8 |
- * wavefronts << 12; 2: tiles of shape
- * fp8_tile_cfg - 1, exp[12] = 1 with the tiles of a column starting at different places of K) */
+ * wavefronts << 12; 2: tiles of shape fp8_tile_cfg - 1) */
 int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb, const float* sa, int64_t sa_row_stride,
                                   int64_t sa_block_stride, const float* sb, int64_t sb_k_stride, int64_t sb_n_stride, const void* bias, void* out,
                                   int64_t ldc, int out_dtype, int64_t size_m, int64_t size_n, int64_t size_k, void* stream,
