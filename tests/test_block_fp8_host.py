@@ -209,3 +209,42 @@ def test_rope_refusals():
     for fields, text in ((dict(d=100, rotary=16, ld=1000), "head_dim"), (dict(d=520, ld=5200), "head_dim"), (dict(rotary=24), "rotary_dim")):
         refused("vaq_qk_norm_rope", with_(base, **fields), NOT_BUILT, text)
     assert _lib.load().vaq_qk_norm_rope(*with_(base, tokens=0, qkv=None)) == 0
+
+
+# ------------------------------------------------------------------------------------------------ plans of the product
+
+def test_prices_are_those_of_the_fit_and_choose_well():
+    """profiles/plan_prices/fp8_block.py restates the prices: the library's plan is the cheapest of its, at its price; on the recorded times the choice is near the best."""
+    import importlib.util
+    import os
+
+    import numpy as np
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "plan_prices", "fp8_block.py")
+    spec = importlib.util.spec_from_file_location("fp8_block_prices", path)
+    f = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(f)
+    few, tiles = f.tables()
+    assert [len(r) for r in few.values()] == [9] * 4 and [len(r) for r in tiles] == [8] * 6
+    _, by_problem = f.load()
+    problems = list(by_problem)[:300]
+    assert f.choice({p: by_problem[p] for p in problems}, few, tiles).mean() < 1.03
+    lib, plan = _lib.load(), (ctypes.c_double * 6)()
+    for m, k, n in problems[:100]:
+        assert lib.vaq_fp8_block_plan(m, n, k, plan) == 0
+        mb, j, ahead, waves, shape = map(int, plan[:5])
+        name = f"r{mb}.{j}.{ahead}.{waves}" if mb else f"t{shape}"
+        at = [np.array([float(x)]) for x in (m, k, n)]
+        assert float(f.price(name, few, tiles, *at)[0]) == pytest.approx(plan[5], rel=1e-9)
+        for other in by_problem[m, k, n]:
+            assert float(f.price(other, few, tiles, *at)[0]) >= plan[5] * (1 - 1e-9)
+
+
+def test_every_plan_in_reach_is_built():
+    """The cheapest plan of small, large and odd problems is one that the launch takes (a plan that is not built would be refused at its call)."""
+    lib, plan = _lib.load(), (ctypes.c_double * 6)()
+    for m in (1, 15, 17, 48, 64, 100, 333, 1024, 1025, 8192):
+        for k in (16, 512, 2976, 14336, 131072):
+            for n in (16, 144, 4096, 28672, 262144):
+                assert lib.vaq_fp8_block_plan(m, n, k, plan) == 0 and plan[5] > 0
+                mb, j, ahead, waves, shape = map(int, plan[:5])
+                assert (mb == 0 and 0 <= shape < 6) or ((mb + ahead * j) * waves < 40 and j in (1, 2, 4) and (waves == 4 or j == 1) and (j < 4 or ahead == 1))

@@ -69,6 +69,7 @@ _SIGNATURES = {
                                              c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
     "vaq_fp8_block_scaled_mm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                         c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    "vaq_fp8_block_plan": (c_int, [c_int64, c_int64, c_int64, POINTER(ctypes.c_double)]),
     "vaq_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p]),
 }

@@ -39,6 +39,7 @@ constexpr uint32_t F8B_NOWHERE = 0x80000000u;      // an offset past every opera
 struct F8bRows {
   int mb = 0, j = 0, ahead = 0, waves = 0;
 };
+size_t fp8_block_rows_lds_bytes(int64_t K, const F8bRows& r);
 bool fp8_block_rows_fits(int64_t K, const F8bRows& r);
 bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, const F8bRows& r, hipStream_t s);
 // tiles (fp8_block_tile_kernel.h)

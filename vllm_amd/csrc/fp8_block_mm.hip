@@ -1,6 +1,8 @@
 // FP8 product with a scale for each block of 128 (fp8_block_mm.h): arguments, choice of the kernel, launch of the tiles.
 #include "fp8_block_tile_kernel.h"
 
+#include <math.h>
+
 namespace vaq {
 
 template <int BM, int BN, int WAVES, typename Kernel>
@@ -42,26 +44,88 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStre
   return bf16 ? launch_type<true>(p, shape, s) : launch_type<false>(p, shape, s);
 }
 
-// The kernel of a problem.
+// ----------------------------------------------------------------------------- choice of the kernel
+// The cheapest plan by price, in us.  Rows: a step is a latency, the bytes into the compute unit or the products, whichever is longest; a workgroup is its start, its steps and its
+// meeting; beside all of them the weights from memory, once and a share for every further block of rows.  Tiles: rounds of workgroups (a last, partly filled one costs a share of
+// a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 9891
+// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 2967 that the fit had not seen the cheapest plan takes 1.013 of the fastest one's time
+// in the mean; without eight wavefronts 1.019, without any one of the tile shapes 1.016 .. 1.027.  (profiles/plan_prices/fp8_block.py)
+constexpr double ROWS_PRICE[4][9] = {      // by steps ahead and wavefronts: 1, 4; 1, 8; 2, 4; 2, 8
+    {0.7175, 0.2233, 0.08537, 0.5477, 0.1458, 0.2031, 0.3329, 1.852, 1.326e-07},
+    {0.6447, 0.1456, 0.2614, 0.8933, 2.161e-09, 0.2047, 0.4566, 1.853, 0.6736},
+    {0.4789, 0.2017, 0.1329, 1.073, 0.07598, 0.21, 0.3385, 1.632, 0.3615},
+    {0.1219, 0.1974, 0.01679, 1.342, 5.481e-09, 0.2228, 0.4273, 1.603, 0.5403},
+};
+constexpr double TILE_PRICE[F8B_SHAPES][8] = {
+    {0.801, 2.021, 0.2395, 0.2008, 0.2297, 2.067, 0.4606, 0.1698},
+    {0.8389, 1.406, 0.3627, 0.2204, 0.1846, 2.792, 0.79, 0.2233},
+    {0.7977, 2.238, 0.5305, 0.2131, 0.1959, 2.736, 0.334, 0.1353},
+    {0.7573, 2.982, 0.8615, 0.2674, 0.02411, 3.191, 0.2571, 0.1805},
+    {0.7526, 4.047, 0.8291, 0.1418, 1.137e-06, 2.734, 0.1566, 0.08221},
+    {0.816, 5.459, 1.417, 0.2169, 0.2788, 2.903, 0.1247, 0.05883},
+};
+constexpr int TILE_ROWS[F8B_SHAPES] = {64, 64, 128, 128, 256, 256}, TILE_COLUMNS[F8B_SHAPES] = {64, 128, 128, 256, 128, 256};
+static double cubes(double a, double b, double c = 0) { return cbrt(a * a * a + b * b * b + c * c * c); }
+
+static double rows_us(const F8bRows& r, double M, double N, double K, int cus) {
+  const double* const c = ROWS_PRICE[(r.ahead - 1) * 2 + (r.waves == 8)];
+  const double blocks = ceil(M / 16 / r.mb), per_cu = ceil(ceil(N / 16 / r.j) * blocks / cus);
+  const double slots = fmin(floor(160.0 * 1024 / fp8_block_rows_lds_bytes((int64_t)K, r)), 16 / r.waves), w = r.waves / 4.0;
+  const double side = fmin(per_cu, slots) * w, rounds = fmax(per_cu / slots, 1.0);
+  const double step = cubes(c[0], c[1] * side * (r.mb + r.j), c[2] * side * r.mb * r.j);
+  const double core = rounds * (c[3] + ceil(ceil(K / 256) / r.waves) * step + c[4] * r.mb * r.j * w);
+  return c[7] + cubes(core, c[5] * 1e-6 * K * N * (1 + c[6] * (blocks - 1))) + c[8] * 1e-6 * M * N;
+}
+static double tile_us(int shape, double M, double N, double K, int cus) {
+  const double* const c = TILE_PRICE[shape];
+  const double down = ceil(M / TILE_ROWS[shape]), across = ceil(N / TILE_COLUMNS[shape]);
+  const double full = floor(down * across / cus), rest = down * across / cus - full;
+  const double rounds = full + (rest > 0 ? c[0] + (1 - c[0]) * rest : 0);
+  const double core = rounds * (c[1] + ceil(K / F8B) * c[2] * (1 + c[7] / down));
+  return c[5] + cubes(core, c[3] * 1e-6 * K * N * (1 + c[4] * (down - 1))) + c[6] * 1e-6 * M * N;
+}
+
 struct F8bPlan {
   F8bRows rows;      // mb = 0: tiles
   int shape = 0;
+  double us = -1;
 };
-static F8bPlan plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
-  F8bPlan plan;
+constexpr int64_t ROWS_MAX_M = 1024;      // (beyond, a problem is many tiles)
+static F8bPlan cheapest(int64_t M, int64_t N, int64_t K, int cus, bool rows_ok) {
+  F8bPlan best;
+  auto offer = [&](const F8bRows& r, int shape, double us) {
+    if (best.us >= 0 && best.us <= us) return;
+    best.rows = r;
+    best.shape = shape;
+    best.us = us;
+  };
+  for (int shape = 0; shape < F8B_SHAPES; ++shape) offer(F8bRows{}, shape, tile_us(shape, (double)M, (double)N, (double)K, cus));
+  if (rows_ok && M <= ROWS_MAX_M)
+    for (int mb = 1; mb <= 4 && (mb == 1 || M > 16 * (mb - 1)); ++mb)
+      for (int j = 1; j <= 4; j *= 2)
+        for (int ahead = 1; ahead <= 2; ++ahead)
+          for (int waves = 4; waves <= 8; waves += 4)
+            if (const F8bRows r{mb, j, ahead, waves}; M <= 128 * mb && fp8_block_rows_fits(K, r)) offer(r, 0, rows_us(r, (double)M, (double)N, (double)K, cus));
+  return best;
+}
+// Plans of recent problems, by size (a search costs 3 us).  Direct mapped, one table per thread.
+static const F8bPlan& plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
+  struct Entry {
+    int64_t M = -1, N = 0, K = 0;
+    int cus = 0;
+    bool rows_ok = false;
+    F8bPlan plan;
+  };
+  static thread_local Entry table[256];
   const int cus = num_cus_current_device();
-  if (rows_ok && M <= 64) {
-    const int mb = (int)((M + 15) / 16);
-    // as many n-tiles a workgroup as leave every compute unit one
-    for (int j = 4; j >= 1; j /= 2)
-      if (const F8bRows r{mb, j, 2, 4}; fp8_block_rows_fits(K, r) && (j == 1 || (N + 16 * j - 1) / (16 * j) >= cus)) {
-        plan.rows = r;
-        return plan;
-      }
+  const uint64_t h = (uint64_t)M * 0x9e3779b97f4a7c15ull ^ (uint64_t)N * 0xc2b2ae3d27d4eb4full ^ (uint64_t)K * 0x165667b19e3779f9ull;
+  Entry& e = table[h >> 56];
+  if (e.M != M || e.N != N || e.K != K || e.cus != cus || e.rows_ok != rows_ok) {
+    e.M = -1;
+    e.plan = cheapest(M, N, K, cus, rows_ok);
+    e.N = N; e.K = K; e.cus = cus; e.rows_ok = rows_ok; e.M = M;
   }
-  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  plan.shape = tiles(256, 256) >= cus ? 5 : tiles(128, 256) >= cus ? 3 : tiles(128, 128) >= cus / 2 ? 2 : tiles(64, 128) >= cus / 2 ? 1 : 0;
-  return plan;
+  return e.plan;
 }
 
 static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
@@ -127,4 +191,12 @@ extern "C" int vaq_fp8_block_scaled_mm(const uint8_t* a, int64_t lda, const uint
                                        int64_t ldc, int out_dtype, int64_t size_m, int64_t size_n, int64_t size_k, void* stream) {
   return vaq_fp8_block_scaled_mm_tuned(a, lda, b, ldb, sa, sa_row_stride, sa_block_stride, sb, sb_k_stride, sb_n_stride, bias, out, ldc, out_dtype, size_m,
                                        size_n, size_k, stream, nullptr);
+}
+
+extern "C" int vaq_fp8_block_plan(int64_t size_m, int64_t size_n, int64_t size_k, double* plan) {
+  VAQ_CHECK_ARG(plan && size_m > 0 && size_n > 0 && size_k > 0, "fp8_block_plan: no problem");
+  const F8bPlan p = cheapest(size_m, size_n, size_k, num_cus_current_device(), true);
+  const double out[6] = {(double)p.rows.mb, (double)p.rows.j, (double)p.rows.ahead, (double)p.rows.waves, (double)p.shape, p.us};
+  for (int i = 0; i < 6; ++i) plan[i] = out[i];
+  return VAQ_OK;
 }

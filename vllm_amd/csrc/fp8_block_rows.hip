@@ -3,6 +3,7 @@
 
 namespace vaq {
 
+size_t fp8_block_rows_lds_bytes(int64_t K, const F8bRows& r) { return f8br_lds_bytes(K, r.mb, r.j, r.ahead, r.waves); }
 bool fp8_block_rows_fits(int64_t K, const F8bRows& r) { return f8br_built(r.mb, r.j, r.ahead, r.waves) && f8br_lds_bytes(K, r.mb, r.j, r.ahead, r.waves) <= 160 * 1024; }
 
 template <bool BF16, int MB, int J, int AHEAD, int NW, bool TAIL>

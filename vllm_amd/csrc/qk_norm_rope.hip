@@ -32,11 +32,45 @@ __device__ inline void unpack(v4u r, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = F16Traits<BF16>::to_float((uint16_t)(w[i / 2] >> (16 * (i & 1))));
 }
 
+// The sum over groups of 2^log2 lanes, in every lane of the group, in registers: pairs inside four lanes, mirrors of 8 and 16, swaps of rows of 16 and of halves.
+__device__ inline float group_sum(float v, int log2) {
+  auto f = [](auto u) { return __builtin_bit_cast(float, (uint32_t)u); };
+  auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
+  if (log2 > 0) v += f(__builtin_amdgcn_mov_dpp((int)u(v), 0xb1, 0xf, 0xf, true));       // quad_perm 1 0 3 2
+  if (log2 > 1) v += f(__builtin_amdgcn_mov_dpp((int)u(v), 0x4e, 0xf, 0xf, true));       // quad_perm 2 3 0 1
+  if (log2 > 2) v += f(__builtin_amdgcn_mov_dpp((int)u(v), 0x141, 0xf, 0xf, true));      // row_half_mirror
+  if (log2 > 3) v += f(__builtin_amdgcn_mov_dpp((int)u(v), 0x140, 0xf, 0xf, true));      // row_mirror
+  if (log2 > 4) {
+    const auto s = __builtin_amdgcn_permlane16_swap(u(v), u(v), false, false);
+    v = f(s[0]) + f(s[1]);
+  }
+  if (log2 > 5) {
+    const auto s = __builtin_amdgcn_permlane32_swap(u(v), u(v), false, false);
+    v = f(s[0]) + f(s[1]);
+  }
+  return v;
+}
+
+// N consecutive numbers of a row of cos and sin, aligned to their type only
+template <bool CACHE32, bool BF16, int N>
+__device__ inline void angles(const void* row, int at, float (&to)[8], int first) {
+  if constexpr (CACHE32) {
+    typedef float vec __attribute__((ext_vector_type(N), aligned(4)));
+    const vec v = *reinterpret_cast<const vec*>((const float*)row + at);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[first + i] = v[i];
+  } else {
+    typedef uint16_t vec __attribute__((ext_vector_type(N), aligned(2)));
+    const vec v = *reinterpret_cast<const vec*>((const uint16_t*)row + at);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[first + i] = F16Traits<BF16>::to_float(v[i]);
+  }
+}
+
 template <bool BF16, bool CACHE32, bool HALVES>
 __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
   using T = F16Traits<BF16>;
   const int64_t token = blockIdx.x, position = p.positions[token];
-  if (position < 0 || position >= p.cache_rows) return;      // not a token of a sequence: its rows stay as they are
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lanes = 1 << p.lanes_log2, per_wave = 64 >> p.lanes_log2;
   const int e = (lane & (lanes - 1)) * 8;      // first of this lane's values in a head
@@ -55,49 +89,67 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
     }
   };
   int round = wave;
-  request(round);
+  request(round);      // (ahead of the wait for the position)
+  v4u raw_q = {0u, 0u, 0u, 0u}, raw_k = {0u, 0u, 0u, 0u};
+  if (in_head) {
+    raw_q = *reinterpret_cast<const v4u*>(p.q_weight + e);
+    raw_k = *reinterpret_cast<const v4u*>(p.k_weight + e);
+  }
+  if (position < 0 || position >= p.cache_rows) return;      // not a token of a sequence: its rows stay as they are
 
-  // cos and sin of this lane's values; values that are not rotated have cos 1 and sin 0
-  float c[8], s[8], wq[8] = {}, wk[8] = {};
+  // cos and sin of this lane's values; values that are not rotated have cos 1 and sin 0.  The second of a pair has + sin, the first - sin.
+  float c[8], s[8], wq[8], wk[8];
   const int half = p.rotary / 2;
+  const void* const angle = (const char*)p.cache + position * p.cache_stride * (CACHE32 ? 4 : 2);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     c[i] = 1.f;
     s[i] = 0.f;
-    if (e + i < p.rotary) {
-      const int at = HALVES ? (e >= half ? e - half : e) + i : (e + i) / 2;
-      if constexpr (CACHE32) {
-        const float* const angle = (const float*)p.cache + position * p.cache_stride;
-        c[i] = angle[at];
-        s[i] = angle[half + at];
-      } else {
-        const uint16_t* const angle = (const uint16_t*)p.cache + position * p.cache_stride;
-        c[i] = T::to_float(angle[at]);
-        s[i] = T::to_float(angle[half + at]);
+  }
+  if constexpr (HALVES) {
+    if (e < p.rotary) {      // (both halves are whole lanes)
+      const int at = e >= half ? e - half : e;
+      angles<CACHE32, BF16, 8>(angle, at, c, 0);
+      angles<CACHE32, BF16, 8>(angle, half + at, s, 0);
+      if (e < half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = -s[i];
       }
-      // the second of a pair has + sin, the first - sin
-      if (HALVES ? e < half : !(i & 1)) s[i] = -s[i];
     }
+  } else {
+    float cc[8], ss[8];
+    if (e + 8 <= p.rotary) {
+      angles<CACHE32, BF16, 4>(angle, e / 2, cc, 0);
+      angles<CACHE32, BF16, 4>(angle, half + e / 2, ss, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e + 2 * i < p.rotary) {
+        if (e + 8 > p.rotary) {      // the last rotated values end inside the lane's
+          angles<CACHE32, BF16, 1>(angle, e / 2 + i, cc, i);
+          angles<CACHE32, BF16, 1>(angle, half + e / 2 + i, ss, i);
+        }
+        c[2 * i] = c[2 * i + 1] = cc[i];
+        s[2 * i] = -ss[i];
+        s[2 * i + 1] = ss[i];
+      }
   }
-  if (in_head) {
-    unpack<BF16>(*reinterpret_cast<const v4u*>(p.q_weight + e), wq);
-    unpack<BF16>(*reinterpret_cast<const v4u*>(p.k_weight + e), wk);
-  }
-  // (HALVES: both halves of the rotated values are whole lanes)
+  unpack<BF16>(raw_q, wq);
+  unpack<BF16>(raw_k, wk);
   const int partner = !HALVES || e >= p.rotary ? lane : e < half ? lane + half / 8 : lane - half / 8;
+  const float over_dim = 1.0f / (float)p.head_dim;
 
   for (; round < rounds; round += QK_AHEAD * (QK_T / 64)) {
     if (round != wave) request(round);
 #pragma unroll
     for (int i = 0; i < QK_AHEAD; ++i) {
-      const int h = head_of(round + i * (QK_T / 64));
       if (round + i * (QK_T / 64) >= rounds) break;      // (the same for the whole wavefront)
+      const int h = head_of(round + i * (QK_T / 64));
       float y[8], ss = 0.f;
       unpack<BF16>(x[i], y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
-      for (int d = 1; d < lanes; d *= 2) ss += __shfl_xor(ss, d);
-      const float rms = rsqrtf(ss / (float)p.head_dim + p.eps);
+      const float rms = rsqrtf(group_sum(ss, p.lanes_log2) * over_dim + p.eps);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = y[j] * rms * (h < p.heads_q ? wq[j] : wk[j]);
       float z[8];

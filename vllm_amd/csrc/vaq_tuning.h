@@ -78,6 +78,9 @@ int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, const uint8_t* 
                                   int64_t ldc, int out_dtype, int64_t size_m, int64_t size_n, int64_t size_k, void* stream,
                                   const VaqTuning* tuning);
 
+/* The plan of a block-scaled FP8 product: plan[0 .. 5] = blocks of 16 rows (0: tiles), n-tiles, steps that weights are ahead, wavefronts, tile shape, predicted us. */
+int vaq_fp8_block_plan(int64_t size_m, int64_t size_n, int64_t size_k, double* plan);
+
 /*
  * The plan of the W4A16 decode kernel for a problem, without launching anything: plan[0 .. 5] = weight tiles per wavefront, K
  * slices and n-tiles per workgroup, parts of K, staged rows, predicted us (negative: no plan).  `sub` = groups per 128
