@@ -16,6 +16,8 @@
 // how the product reads them.
 #include "vaq_common.h"
 
+#include <string.h>
+
 namespace vaq {
 
 namespace {
@@ -104,11 +106,20 @@ __device__ inline void store_codes(uint8_t* to, int left, const float (&y)[8], F
 // Bound by memory: every value is read once.  A workgroup takes 16 rows x 512 columns; 16 rows' scales of a group are 64 contiguous bytes in the
 // package's layout.  Quotients: of 16-bit values the correctly rounded one (div16_exact; the same codes as IEEE division), of fp32 values the
 // IEEE division, of silu(g) u the product with 1 / s, whose second rounding (2^-24) only moves codes of values that near a tie.
+// (What the first requests need arrives in registers with the launch, as one vector: the host's cost of a launch grows with the number of arguments.)
+struct QuantTo {
+  uint8_t* out;
+  int64_t out_stride;
+  float* scales;
+  int64_t scale_row, scale_group;
+};
+__device__ inline int64_t join(uint32_t lo, uint32_t hi) { return (int64_t)((uint64_t)hi << 32 | lo); }
 template <int DT, bool VEC, bool SILU>
-__global__ __launch_bounds__(GQ_T) void group_quant_kernel(const void* __restrict__ in, int64_t in_stride, int64_t rows, int hidden,
-                                                           uint8_t* __restrict__ out, int64_t out_stride, float* __restrict__ scales,
-                                                           int64_t scale_row, int64_t scale_group) {
+__global__ __launch_bounds__(GQ_T) void group_quant_kernel(const v8u head, const QuantTo to) {
   constexpr int SIZE = Raw8<DT>::SIZE;
+  const char* const in = head_ptr<char>(head[0], head[1]);
+  const int64_t in_stride = join(head[2], head[3]), rows = join(head[4], head[5]);
+  const int hidden = (int)head[6];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int e = ((int)blockIdx.x * 64 + lane) * 8, left = hidden - e;
   const int64_t step = (int64_t)gridDim.y * (GQ_T / 64 * GQ_ROWS);
@@ -116,7 +127,7 @@ __global__ __launch_bounds__(GQ_T) void group_quant_kernel(const void* __restric
     Raw8<DT> a[GQ_ROWS], b[SILU ? GQ_ROWS : 1];
 #pragma unroll
     for (int i = 0; i < GQ_ROWS; ++i) {
-      const char* row = (const char*)in + (r0 + i) * in_stride * SIZE;
+      const char* row = in + (r0 + i) * in_stride * SIZE;
       const int n = r0 + i < rows ? left : 0;
       a[i] = load8<DT, VEC>(row, e, n);
       if constexpr (SILU) b[i] = load8<DT, VEC>(row, (int64_t)hidden + e, n);
@@ -135,25 +146,34 @@ __global__ __launch_bounds__(GQ_T) void group_quant_kernel(const void* __restric
         for (int k = 0; k < 8; ++k) y[k] = y[k] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * y[k])) * u[k];
       }
       const float s = scale_of(row16_umax(magnitude(y))), r = 1.0f / s;
-      uint8_t* const to = out + (r0 + i) * out_stride + e;
-      if constexpr (SILU) store_codes<VEC>(to, left, y, [&](float v) { return v * r; });
-      else if constexpr (DT == VAQ_F32) store_codes<VEC>(to, left, y, [&](float v) { return v / s; });
-      else if (s < __builtin_inff()) store_codes<VEC>(to, left, y, [&](float v) { return div16_exact(v, s, r); });
-      else store_codes<VEC>(to, left, y, [&](float v) { return v / s; });
+      uint8_t* const codes = to.out + (r0 + i) * to.out_stride + e;
+      if constexpr (SILU) store_codes<VEC>(codes, left, y, [&](float v) { return v * r; });
+      else if constexpr (DT == VAQ_F32) store_codes<VEC>(codes, left, y, [&](float v) { return v / s; });
+      else if (s < __builtin_inff()) store_codes<VEC>(codes, left, y, [&](float v) { return div16_exact(v, s, r); });
+      else store_codes<VEC>(codes, left, y, [&](float v) { return v / s; });
       mine = (lane & 15) == i ? s : mine;
     }
     const int64_t row = r0 + (lane & 15), g = (int64_t)blockIdx.x * 4 + (lane >> 4);
-    if ((lane & 15) < GQ_ROWS && row < rows && g * GROUP < hidden) scales[row * scale_row + g * scale_group] = mine;
+    if ((lane & 15) < GQ_ROWS && row < rows && g * GROUP < hidden) to.scales[row * to.scale_row + g * to.scale_group] = mine;
   }
 }
 
 // One row a workgroup, which stays in registers from the sum of squares to the codes.  Bound by memory with many rows; with few by one round trip
 // for row, residual and weight (all requested together) and one meeting of the wavefronts.
+struct NormTo {
+  uint8_t* out;
+  float* scales;
+  int64_t scale_row, scale_group;
+  uint16_t* residual_out;
+};
 template <bool BF16, bool VEC, bool RES, int TPB, int NV>
-__global__ __launch_bounds__(TPB) void rms_norm_group_quant_kernel(const uint16_t* input, const uint16_t* residual,
-                                                                   const uint16_t* __restrict__ weight, int64_t in_stride, int hidden, float eps,
-                                                                   uint8_t* __restrict__ out, float* __restrict__ scales, int64_t scale_row,
-                                                                   int64_t scale_group, uint16_t* residual_out) {
+__global__ __launch_bounds__(TPB) void rms_norm_group_quant_kernel(const v8u head, const v2u head2, const NormTo to) {
+  const uint16_t* const input = head_ptr<uint16_t>(head[0], head[1]);
+  const uint16_t* const residual = head_ptr<uint16_t>(head[2], head[3]);
+  const uint16_t* const weight = head_ptr<uint16_t>(head[4], head[5]);
+  const int64_t in_stride = join(head[6], head[7]);
+  const int hidden = (int)head2[0];
+  const float eps = __builtin_bit_cast(float, (uint32_t)head2[1]);
   constexpr int DT = BF16 ? VAQ_BF16 : VAQ_F16;
   using T = F16Traits<BF16>;
   __shared__ float smem[TPB / 64];
@@ -185,15 +205,15 @@ __global__ __launch_bounds__(TPB) void rms_norm_group_quant_kernel(const uint16_
         x[v][i] += r[i];
         z[i] = T::from_float(x[v][i]);
       }
-      uint16_t* const to = residual_out + row * hidden + e;
+      uint16_t* const sum = to.residual_out + row * hidden + e;
       if constexpr (VEC) {
         if (e < hidden)
-          *reinterpret_cast<v4u*>(to) = v4u{(uint32_t)z[0] | (uint32_t)z[1] << 16, (uint32_t)z[2] | (uint32_t)z[3] << 16,
+          *reinterpret_cast<v4u*>(sum) = v4u{(uint32_t)z[0] | (uint32_t)z[1] << 16, (uint32_t)z[2] | (uint32_t)z[3] << 16,
                                             (uint32_t)z[4] | (uint32_t)z[5] << 16, (uint32_t)z[6] | (uint32_t)z[7] << 16};
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (e + i < hidden) to[i] = z[i];
+          if (e + i < hidden) sum[i] = z[i];
       }
     }
 #pragma unroll
@@ -209,8 +229,8 @@ __global__ __launch_bounds__(TPB) void rms_norm_group_quant_kernel(const uint16_
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = e + i < hidden ? x[v][i] * rms * w[i] : 0.f;      // (0 * infinity behind the row)
     const float s = scale_of(row16_umax(magnitude(y))), r = 1.0f / s;
-    store_codes<VEC>(out + row * hidden + e, hidden - e, y, [&](float f) { return f * r; });
-    if ((c & 15) == 0 && e < hidden) scales[row * scale_row + (int64_t)(c >> 4) * scale_group] = s;
+    store_codes<VEC>(to.out + row * hidden + e, hidden - e, y, [&](float f) { return f * r; });
+    if ((c & 15) == 0 && e < hidden) to.scales[row * to.scale_row + (int64_t)(c >> 4) * to.scale_group] = s;
   }
 }
 
@@ -219,8 +239,11 @@ void launch_quant(bool vec, const void* in, int64_t in_stride, int64_t rows, int
                   int64_t scale_row, int64_t scale_group, hipStream_t s) {
   const int64_t row_blocks = (rows + GQ_T / 64 * GQ_ROWS - 1) / (GQ_T / 64 * GQ_ROWS);
   const dim3 grid((unsigned)((hidden + 511) / 512), (unsigned)(row_blocks < 65535 ? row_blocks : 65535));
-  if (vec) group_quant_kernel<DT, true, SILU><<<grid, GQ_T, 0, s>>>(in, in_stride, rows, (int)hidden, out, out_stride, scales, scale_row, scale_group);
-  else group_quant_kernel<DT, false, SILU><<<grid, GQ_T, 0, s>>>(in, in_stride, rows, (int)hidden, out, out_stride, scales, scale_row, scale_group);
+  const uint64_t in_s = (uint64_t)in_stride, n = (uint64_t)rows;
+  const v8u head{ptr_lo(in), ptr_hi(in), (uint32_t)in_s, (uint32_t)(in_s >> 32), (uint32_t)n, (uint32_t)(n >> 32), (uint32_t)hidden, 0u};
+  const QuantTo to{out, out_stride, scales, scale_row, scale_group};
+  if (vec) group_quant_kernel<DT, true, SILU><<<grid, GQ_T, 0, s>>>(head, to);
+  else group_quant_kernel<DT, false, SILU><<<grid, GQ_T, 0, s>>>(head, to);
 }
 
 struct NormArgs {
@@ -235,12 +258,14 @@ struct NormArgs {
 template <bool BF16, bool VEC, int TPB, int NV>
 void launch_norm(const NormArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.tokens);
-  if (a.residual)
-    rms_norm_group_quant_kernel<BF16, VEC, true, TPB, NV><<<grid, TPB, 0, s>>>(a.input, a.residual, a.weight, a.in_stride, (int)a.hidden, a.eps, a.out,
-                                                                             a.scales, a.scale_row, a.scale_group, a.residual_out);
-  else
-    rms_norm_group_quant_kernel<BF16, VEC, false, TPB, NV><<<grid, TPB, 0, s>>>(a.input, a.residual, a.weight, a.in_stride, (int)a.hidden, a.eps, a.out,
-                                                                              a.scales, a.scale_row, a.scale_group, a.residual_out);
+  const uint64_t in_s = (uint64_t)a.in_stride;
+  const v8u head{ptr_lo(a.input), ptr_hi(a.input), ptr_lo(a.residual), ptr_hi(a.residual), ptr_lo(a.weight), ptr_hi(a.weight), (uint32_t)in_s, (uint32_t)(in_s >> 32)};
+  uint32_t eps_bits;
+  memcpy(&eps_bits, &a.eps, sizeof(eps_bits));
+  const v2u head2{(uint32_t)a.hidden, eps_bits};
+  const NormTo to{a.out, a.scales, a.scale_row, a.scale_group, a.residual_out};
+  if (a.residual) rms_norm_group_quant_kernel<BF16, VEC, true, TPB, NV><<<grid, TPB, 0, s>>>(head, head2, to);
+  else rms_norm_group_quant_kernel<BF16, VEC, false, TPB, NV><<<grid, TPB, 0, s>>>(head, head2, to);
 }
 constexpr int64_t NORM_MAX = 1024 * 8 * 8;      // values of a row that a workgroup holds
 template <bool BF16>
