@@ -198,6 +198,14 @@ def test_mm_plans_that_are_not_built():
     refused("vaq_fp8_block_scaled_mm_tuned", [*base.values(), ctypes.byref(t)], NOT_BUILT, "few rows")
 
 
+def test_mm_of_more_than_a_launch():
+    base = dict(a=P, lda=16, b=P, ldb=16, sa=P, sar=1, sab=8, sb=P, sbk=1, sbn=2, bias=None, out=P, ldc=16, dtype=_lib.VAQ_BF16, m=(1 << 31) - 16, n=16, k=16, stream=None)
+    refused("vaq_fp8_block_scaled_mm", base.values(), NOT_BUILT, "threads")
+    t = _lib.VaqTuning()
+    t.fp8_path, t.fp8_tile_cfg = 2, 1
+    refused("vaq_fp8_block_scaled_mm_tuned", [*with_(base, m=1 << 29), ctypes.byref(t)], NOT_BUILT, "threads")
+
+
 def test_rope_refusals():
     base = dict(qkv=P, ld=768, q=P, k=P, hq=4, hk=1, d=128, eps=1e-6, wq=P, wk=P, cs=P, cs_dtype=_lib.VAQ_F32, cs_ld=128, cs_rows=9, rotary=128, inter=0, pos=P,
                 dtype=_lib.VAQ_BF16, tokens=3, stream=None)

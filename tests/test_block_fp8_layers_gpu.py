@@ -143,3 +143,13 @@ def test_bad_arguments_are_refused_by_both_routes(device):
             call()
     with pytest.raises(NotImplementedError, match="float8_e4m3fn"):
         ops.block_scaled_mm(q.view(torch.uint8), w, s, sw, torch.bfloat16)
+
+
+def test_linear_of_the_last_token_of_each_sequence(device):
+    from vllm_amd import _custom_ops as ops
+    x = torch.randn((3, 5, 256), device=device).to(torch.bfloat16)
+    w = (torch.randn((144, 256), device=device) * 40).to(FP8).t()
+    sw = torch.rand((2, 2), device=device)
+    got = ops.block_fp8_linear(x[:, -1:], w, sw, torch.bfloat16, None)
+    assert got.shape == (3, 1, 144)
+    assert torch.equal(got, ops.block_fp8_linear(x[:, -1:].contiguous(), w, sw, torch.bfloat16, None))

@@ -225,3 +225,16 @@ def test_a_block_of_operators(device):
     q, s = ops.silu_and_mul_group_quant(gate_up)
     down = linear(q, s, weight(hidden, ffn))
     assert bool(down.isfinite().all())
+
+
+def test_strides_of_single_rows_and_blocks_say_nothing(device):
+    from vllm_amd import _custom_ops as ops
+    w = (torch.randn((32, 256), device=device) * 40).to(torch.float8_e4m3fn).t()
+    sw = torch.rand((2, 1), device=device)
+    a = (torch.randn((7, 256), device=device) * 40).to(torch.float8_e4m3fn)
+    sa = torch.rand((7, 2), device=device)
+    far = sa[:1].as_strided((1, 2), (1 << 33, 1))
+    assert torch.equal(ops.block_scaled_mm(a[:1], w, far, sw, torch.float16), ops.block_scaled_mm(a[:1], w, sa[:1], sw, torch.float16))
+    one = sa.as_strided((7, 1), (2, 1 << 33))
+    assert torch.equal(ops.block_scaled_mm(a[:, :128], w[:128], one, sw[:1].as_strided((1, 1), (1 << 33, 1)), torch.float16),
+                       ops.block_scaled_mm(a[:, :128], w[:128], sa[:, :1], sw[:1], torch.float16))

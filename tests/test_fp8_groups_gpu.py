@@ -207,3 +207,40 @@ def test_group_operators_in_a_graph(device):
         for a, b in zip(held, work()):
             assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
         torch.cuda.synchronize()
+
+
+def test_rows_one_stride_apart_in_more_dimensions(device):
+    from vllm_amd import _custom_ops as ops
+    held = _randn((3, 4, 1040), 5, torch.bfloat16).to(device)
+    for x in (held[:, -1:, :512], held[:, :, :520], held[:, :1]):
+        flat = x.reshape(-1, x.shape[-1])
+        codes, scales = ops.scaled_fp8_group_quant(x)
+        want, want_scales = ob.group_quant(flat.cpu())
+        assert codes.shape == x.shape and torch.equal(scales.cpu(), want_scales) and torch.equal(_bits(codes.reshape(flat.shape)), _bits(want))
+        for got, same in ((ops.silu_and_mul_group_quant(x), ops.silu_and_mul_group_quant(flat)),
+                          (ops.rms_norm_group_quant(x, held[0, 0, :x.shape[-1]], 1e-6), ops.rms_norm_group_quant(flat, held[0, 0, :x.shape[-1]], 1e-6))):
+            assert got[0].shape[:-1] == x.shape[:-1] and torch.equal(_bits(got[0]).reshape(_bits(same[0]).shape), _bits(same[0])) and torch.equal(got[1], same[1])
+    with pytest.raises(RuntimeError, match="one stride apart"):
+        ops.scaled_fp8_group_quant(held[:, :2, :512])
+
+
+def test_scales_on_top_of_each_other_are_refused(device):
+    x = _randn((4, 256), 6, torch.float16).to(device)
+    codes = torch.empty((4, 256), dtype=torch.float8_e4m3fn, device=device)
+    for scales in (torch.empty((1, 2), device=device).expand(4, 2), torch.empty(8, device=device).as_strided((4, 2), (1, 1)),
+                   torch.empty(8, device=device).as_strided((4, 2), (1, 3))):
+        with pytest.raises(RuntimeError, match="on top of each other"):
+            torch.ops.vllm_amd.scaled_fp8_group_quant(codes, x, scales)
+
+
+def test_norm_of_more_rows_than_a_launch(device):
+    from vllm_amd import _custom_ops as ops
+    edge = 1 << 21
+    x = torch.randn((edge + 5, 8), device=device, generator=torch.Generator(device).manual_seed(7)).to(torch.bfloat16)
+    residual, w = x.flip(0), x[0].clone()
+    before = residual.clone()
+    codes, scales = ops.rms_norm_group_quant(x, w, 1e-6, residual)
+    for rows in (slice(0, 3), slice(edge - 3, edge + 5)):
+        part = before[rows].clone()
+        want, want_scales = ops.rms_norm_group_quant(x[rows].clone(), w, 1e-6, part)
+        assert torch.equal(_bits(codes[rows]), _bits(want)) and torch.equal(scales[rows], want_scales) and torch.equal(residual[rows], part)

@@ -115,3 +115,20 @@ def test_in_a_graph_and_on_another_stream(device):
         for a, b in zip([t.clone() for t in out], work()):
             assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+def test_more_tokens_than_a_launch(device):
+    from vllm_amd import _custom_ops as ops
+    edge = 1 << 22
+    qkv = torch.randn((edge + 3, 24), device=device, generator=torch.Generator(device).manual_seed(8)).to(torch.float16)
+    angle = torch.rand((50, 8), device=device) * 6
+    cache = torch.cat((angle[:, :4].cos(), angle[:, :4].sin()), 1)
+    positions = torch.arange(edge + 3, device=device) % 50
+
+    def work(rows):
+        return ops.qk_norm_rope(qkv[rows], 1, 1, 8, 1e-6, qkv[0, :8].clone(), qkv[1, :8].clone(), cache, positions[rows].clone(), False)
+
+    every = work(slice(None))
+    for rows in (slice(0, 3), slice(edge - 3, edge + 3)):
+        for a, b in zip(every, work(rows)):
+            assert torch.equal(a[rows], b)

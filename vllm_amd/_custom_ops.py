@@ -682,12 +682,11 @@ def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
         return (0, 0) if t.dim() else None
     if t.stride(-1) != 1 and t.size(-1) != 1:
         return None
-    if t.dim() == 2:
-        return t.size(0), t.stride(0)
-    rows = t.numel() // t.size(-1)
-    if t.dim() == 1:
-        return 1, t.size(-1)
-    return (rows, t.size(-1)) if t.is_contiguous() else None
+    try:
+        rows = t.view(-1, t.size(-1))
+    except RuntimeError:
+        return None
+    return rows.size(0), rows.stride(0)
 
 
 def _check_group_quant(who: str, result: torch.Tensor, input: torch.Tensor, scale: torch.Tensor, columns: int,
@@ -703,6 +702,11 @@ def _check_group_quant(who: str, result: torch.Tensor, input: torch.Tensor, scal
     groups = -(-columns // FP8_GROUP)
     _check(scale.dtype == torch.float32 and scale.dim() == 2 and (rows[0] == 0 or tuple(scale.shape) == (rows[0], groups)),
            lambda: f"{who}: scale must be float32 [{rows[0]}, {groups}], one for each group of {FP8_GROUP}")
+    extent = 1
+    for stride, n in sorted(zip(scale.stride(), scale.shape)):
+        if n > 1:
+            _check(stride >= extent, f"{who}: scales lie on top of each other")
+            extent = stride * n
     return rows
 
 

@@ -142,6 +142,10 @@ static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
     plan.shape = t.fp8_tile_cfg - 1;
     VAQ_CHECK_SUPPORTED(plan.shape >= 0 && plan.shape < F8B_SHAPES, "fp8_block_scaled_mm: no such tile shape");
   }
+  const int64_t units = plan.rows.mb > 0 ? (p.M + 16 * (int64_t)plan.rows.mb - 1) / (16 * plan.rows.mb) * ((p.N + 16 * (int64_t)plan.rows.j - 1) / (16 * plan.rows.j))
+                                         : (p.M + (int64_t)TILE_ROWS[plan.shape] - 1) / TILE_ROWS[plan.shape] *
+                                               ((p.N + (int64_t)TILE_COLUMNS[plan.shape] - 1) / TILE_COLUMNS[plan.shape]);
+  VAQ_CHECK_SUPPORTED(units < (1 << 23) - 8, "fp8_block_scaled_mm: M = %d, N = %d need more than a launch's 2^32 threads", p.M, p.N);      // (512 each)
   if (plan.rows.mb > 0) {
     if (!fp8_block_rows_launch(p, bf16, plan.rows, s)) return VAQ_ERR_LAUNCH;
   } else if (const int rc = fp8_block_tile_launch(p, bf16, plan.shape, s); rc != VAQ_OK) {
@@ -170,6 +174,8 @@ extern "C" int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, cons
                 "fp8_block_scaled_mm: row strides lda = %lld, ldb = %lld (multiples of 16, at least K), ldc = %lld (a multiple of 4, at least N)", (long long)lda,
                 (long long)ldb, (long long)ldc);
   const int64_t blocks = (size_k + F8B - 1) / F8B, limit = (int64_t)1 << 31;
+  if (size_m == 1) sa_row_stride = 0;      // (the stride of a single one says nothing)
+  if (blocks == 1) sa_block_stride = sb_k_stride = 0;
   // (a tile is at most 256 rows of each operand: their offsets fit in 31 bits)
   VAQ_CHECK_SUPPORTED(lda <= (1 << 22) && ldb <= (1 << 22), "fp8_block_scaled_mm: rows more than 4 MiB apart are not built (lda = %lld, ldb = %lld)", (long long)lda,
                       (long long)ldb);
@@ -178,8 +184,6 @@ extern "C" int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, cons
                           blocks * sb_k_stride * 4 < limit,
                       "fp8_block_scaled_mm: scales of 256 rows or of a block of columns lie more than 2 GiB apart");
   VAQ_CHECK_SUPPORTED(size_k <= 131072, "fp8_block_scaled_mm: K = %lld, at most 131072 is built", (long long)size_k);      // (the scales of a block of columns are in LDS)
-  const int64_t most = (int64_t)1 << 31;
-  VAQ_CHECK_SUPPORTED(((size_m + 15) / 16) * ((size_n + 15) / 16) < most, "fp8_block_scaled_mm: M = %lld, N = %lld", (long long)size_m, (long long)size_n);
   const Fp8BlockParams p{a, b, sa, sb, (const uint16_t*)bias, (uint16_t*)out, sa_row_stride, sb_n_stride, (uint32_t)sa_block_stride, (uint32_t)sb_k_stride,
                          (uint32_t)lda, (uint32_t)ldb, ldc, (int)size_m, (int)size_n, (int)size_k};
   TuningScope scope(tuning);

@@ -282,6 +282,7 @@ void launch_norm_type(bool vec, const NormArgs& a, hipStream_t s) {
 
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 constexpr int64_t MOST = (int64_t)1 << 30;      // values of a row, tokens
+constexpr int64_t NORM_GRID = (int64_t)1 << 21;      // rows of a launch, whose threads are below 2^32
 
 int quant_common(const char* who, const void* in, int in_dtype, int64_t in_stride, int64_t row_values, uint8_t* out, int64_t out_stride, float* scales,
                  int64_t rows, int64_t hidden) {
@@ -339,10 +340,13 @@ extern "C" int vaq_rms_norm_fp8_group_quant(uint8_t* out, float* scales, int64_t
   VAQ_CHECK_ARG(aligned(weight, 2) && aligned(residual, 2) && aligned(residual_out, 2), "rms_norm_fp8_group_quant: pointers are not aligned to their types");
   const bool vec = hidden % 8 == 0 && aligned(input, 16) && aligned(weight, 16) && aligned(residual, 16) && aligned(residual_out, 16) && aligned(out, 8) &&
                    (tokens == 1 || in_row_stride % 8 == 0);
-  const NormArgs a{(const uint16_t*)input, (const uint16_t*)residual, (const uint16_t*)weight, in_row_stride, tokens, hidden, epsilon, out, scales,
-                   scale_row_stride, scale_group_stride, (uint16_t*)residual_out};
-  if (dtype == VAQ_BF16) launch_norm_type<true>(vec, a, (hipStream_t)stream);
-  else launch_norm_type<false>(vec, a, (hipStream_t)stream);
-  VAQ_CHECK_LAUNCH("rms_norm_fp8_group_quant");
+  for (int64_t t = 0; t < tokens; t += NORM_GRID) {
+    const NormArgs a{(const uint16_t*)input + t * in_row_stride, residual ? (const uint16_t*)residual + t * hidden : nullptr, (const uint16_t*)weight, in_row_stride,
+                     tokens - t < NORM_GRID ? tokens - t : NORM_GRID, hidden, epsilon, out + t * hidden, scales + t * scale_row_stride, scale_row_stride,
+                     scale_group_stride, residual ? (uint16_t*)residual_out + t * hidden : nullptr};
+    if (dtype == VAQ_BF16) launch_norm_type<true>(vec, a, (hipStream_t)stream);
+    else launch_norm_type<false>(vec, a, (hipStream_t)stream);
+    VAQ_CHECK_LAUNCH("rms_norm_fp8_group_quant");
+  }
   return VAQ_OK;
 }

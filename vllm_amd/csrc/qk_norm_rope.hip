@@ -13,6 +13,7 @@ namespace vaq {
 namespace {
 
 constexpr int QK_T = 256, QK_AHEAD = 4;      // threads; rounds of heads that are requested together
+constexpr int64_t QK_GRID = (int64_t)1 << 22;      // tokens of a launch, whose threads are below 2^32
 
 struct QkArgs {
   const uint16_t* qkv;
@@ -207,8 +208,15 @@ extern "C" int vaq_qk_norm_rope(const void* qkv, int64_t qkv_row_stride, void* q
   QkArgs a{(const uint16_t*)qkv, (uint16_t*)q_out, (uint16_t*)k_out, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos_sin, positions, qkv_row_stride,
            cos_sin_row_stride, cos_sin_rows, (int)heads_q, (int)heads_k, (int)head_dim, (int)rotary_dim, 0, epsilon};
   while ((8 << a.lanes_log2) < head_dim) ++a.lanes_log2;
-  if (dtype == VAQ_BF16) launch<true>(a, cos_sin_dtype == VAQ_F32, !interleaved, tokens, (hipStream_t)stream);
-  else launch<false>(a, cos_sin_dtype == VAQ_F32, !interleaved, tokens, (hipStream_t)stream);
-  VAQ_CHECK_LAUNCH("qk_norm_rope");
+  for (int64_t left = tokens; left > 0; left -= QK_GRID) {
+    const int64_t n = left < QK_GRID ? left : QK_GRID;
+    if (dtype == VAQ_BF16) launch<true>(a, cos_sin_dtype == VAQ_F32, !interleaved, n, (hipStream_t)stream);
+    else launch<false>(a, cos_sin_dtype == VAQ_F32, !interleaved, n, (hipStream_t)stream);
+    VAQ_CHECK_LAUNCH("qk_norm_rope");
+    a.qkv += n * a.stride;
+    if (a.q) a.q += n * heads_q * head_dim;
+    if (a.k) a.k += n * heads_k * head_dim;
+    a.positions += n;
+  }
   return VAQ_OK;
 }
