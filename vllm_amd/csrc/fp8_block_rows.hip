@@ -13,7 +13,8 @@ static bool launch(const Fp8BlockParams& p, hipStream_t s) {
   auto kern = fp8_block_rows_kernel<BF16, MB, J, AHEAD, NW, TAIL>;
   static size_t reserved[VAQ_MAX_DEVICES];
   if (reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm") != VAQ_OK) return false;
-  hipLaunchKernelGGL(kern, dim3((ranges * row_blocks + 7) / 8 * 8), dim3(NW * 64), lds, s, p, ranges, row_blocks);
+  hipLaunchKernelGGL(kern, dim3((ranges * row_blocks + 7) / 8 * 8), dim3(NW * 64), lds, s,
+                     v8u{ptr_lo(p.b), ptr_hi(p.b), p.ldb, (uint32_t)p.K, (uint32_t)p.N, (uint32_t)p.M, ranges, row_blocks}, p);
   return true;
 }
 

@@ -4,8 +4,8 @@
 //    K each and share nothing until their sums meet in LDS: no barrier in the K loop, no hand-over between workgroups, no scratch.
 //  * Both operands come by direct-to-LDS loads of 4 rows x 256 contiguous bytes into a piece of LDS of the wavefront's own, activations one step ahead, weights
 //    AHEAD = one or two: two where the weights' way from memory counts, one where the LDS has room for larger results instead.
-//  * A wavefront's scales for all of its K range are requested ahead of the first operands, into LDS of its own: a request behind another is answered behind it,
-//    so that the first step's wait covers them and no step waits for scales.
+//  * A wavefront's scales for all of its K range are requested between the first step's weights and activations, into LDS of its own: a request behind another is
+//    answered behind it, so that the first step's wait covers them and no step waits for scales.
 //  * Rows beyond MB * 16 are a further block of rows with workgroups of their own, side by side on the same XCD, so that they find the weights in its L2.
 #pragma once
 #include "fp8_block_mm.h"
@@ -35,16 +35,20 @@ __host__ __device__ inline F8brUnit f8br_unit(uint32_t block, uint32_t ranges, u
 
 // TAIL: K ends inside a step; of the last one each lane asks for the chunks before K, and the rest of both operands arrives as zeros.
 template <bool BF16, int MB, int J, int AHEAD, int NW, bool TAIL>
-__global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_block_rows_kernel(const Fp8BlockParams p, const uint32_t ranges, const uint32_t row_blocks) {
+__global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_block_rows_kernel(const v8u head, const Fp8BlockParams p) {
   using T = F16Traits<BF16>;
   constexpr int KT = F8BR_STEP, R = (J * MB + NW - 1) / NW, TB = 16 * KT, LI = TB / 1024, U = KT / F8B;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r16 = lane & 15;
+  // (what the first request of the weights needs arrives in registers with the launch)
+  const uint8_t* const weights = head_ptr<uint8_t>(head[0], head[1]);
+  const uint32_t ldb = head[2], ranges = head[6], row_blocks = head[7];
+  const int K = (int)head[3], N = (int)head[4], M = (int)head[5];
   const F8brUnit unit = f8br_unit(blockIdx.x, ranges, row_blocks);
   if (unit.range >= ranges) return;
   const int n0 = (int)unit.range * J * 16, row0 = (int)unit.rows * MB * 16;
-  const uint32_t rows = (uint32_t)min(MB * 16, p.M - row0), columns = (uint32_t)min(J * 16, p.N - n0);
-  const int all = (p.K + KT - 1) / KT, per = f8br_steps(p.K, NW), first = w * per, last = min(first + per, all);      // this wavefront's steps
+  const uint32_t rows = (uint32_t)min(MB * 16, M - row0), columns = (uint32_t)min(J * 16, N - n0);
+  const int all = (K + KT - 1) / KT, per = f8br_steps(K, NW), first = w * per, last = min(first + per, all);      // this wavefront's steps
 
   typedef __attribute__((address_space(3))) void* lds_ptr_t;
   const int scales_a = f8br_scales_a(per, MB), scales_b = f8br_scales_b(per);
@@ -52,23 +56,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
   float* const sa_lds = reinterpret_cast<float*>(mine + f8br_operand_bytes(MB, J, AHEAD));
   float* const sb_lds = sa_lds + scales_a;
 
-  // scales: [block of K][row], then [block of K]; blocks past K and past this wavefront's arrive as zeros
-  const int blocks = (p.K + F8B - 1) / F8B, kb0 = first * U, kb_n = max(0, min(last * U, blocks) - kb0);
-  {
-    const __amdgpu_buffer_rsrc_t rsa = f8b_rsrc(p.sa + (int64_t)row0 * p.sa_row, 0x7ffffffcu), rsb = f8b_rsrc(p.sb + (int64_t)(n0 / F8B) * p.sb_n, 0x7ffffffcu);
-    for (int i = 0; i < scales_a; i += 64) {
-      const int kb = (i + lane) / (MB * 16), row = (i + lane) % (MB * 16);
-      const uint32_t at = (uint32_t)min(row, (int)rows - 1) * (uint32_t)p.sa_row * 4u + (uint32_t)(kb0 + kb) * p.sa_block * 4u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)(sa_lds + i), 4, (int)(kb < kb_n ? at : F8B_NOWHERE), 0, 0, 0);
-    }
-    for (int i = 0; i < scales_b; i += 64)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (lds_ptr_t)(sb_lds + i), 4, (int)(i + lane < kb_n ? (uint32_t)(kb0 + i + lane) * p.sb_block * 4u : F8B_NOWHERE), 0, 0, 0);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-
   // a load fetches four whole rows of a tile of 16; their 16-byte chunk c is at place c ^ row: the 16 rows of an operand read hit all banks
-  const uint32_t a_extent = (rows - 1) * p.lda + (uint32_t)p.K, b_extent = (columns - 1) * p.ldb + (uint32_t)p.K, rest = (uint32_t)p.K % KT;
-  const uint8_t *const a = p.a + (int64_t)row0 * p.lda, *const b = p.b + (int64_t)n0 * p.ldb;
+  const uint32_t a_extent = (rows - 1) * p.lda + (uint32_t)K, b_extent = (columns - 1) * ldb + (uint32_t)K, rest = (uint32_t)K % KT;
+  const uint8_t *const a = p.a + (int64_t)row0 * p.lda, *const b = weights + (int64_t)n0 * ldb;
   uint32_t vo_a[LI * MB], vo_w[LI];
 #pragma unroll
   for (int i = 0; i < LI * MB; ++i) {
@@ -78,7 +68,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
 #pragma unroll
   for (int i = 0; i < LI; ++i) {
     const int r = i * 4 + q;
-    vo_w[i] = (uint32_t)r * p.ldb + (uint32_t)((r16 ^ r) * 16);
+    vo_w[i] = (uint32_t)r * ldb + (uint32_t)((r16 ^ r) * 16);
   }
   // A step past the last has no extent and starts at 0 (vaq_common.h): its requests fetch nothing and keep the count of requests under way.
   auto place = [&](uint32_t vo, int r, int g) {
@@ -95,11 +85,23 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
     const __amdgpu_buffer_rsrc_t rb = f8b_rsrc(b, g < last ? b_extent : 0u);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int so = g < last ? (int)(min((uint32_t)(j * 16), columns - 16) * p.ldb + (uint32_t)(g * KT)) : 0;
+      const int so = g < last ? (int)(min((uint32_t)(j * 16), columns - 16) * ldb + (uint32_t)(g * KT)) : 0;
 #pragma unroll
       for (int i = 0; i < LI; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(mine + (MB + s * J + j) * TB + i * 1024), 16, (int)place(vo_w[i], i * 4 + q, g), so, 0, 2);
     }
+  };
+  // scales: [block of K][row], then [block of K]; blocks past K and past this wavefront's arrive as zeros
+  const int blocks = (K + F8B - 1) / F8B, kb0 = first * U, kb_n = max(0, min(last * U, blocks) - kb0);
+  auto load_scales = [&] {
+    const __amdgpu_buffer_rsrc_t rsa = f8b_rsrc(p.sa + (int64_t)row0 * p.sa_row, 0x7ffffffcu), rsb = f8b_rsrc(p.sb + (int64_t)(n0 / F8B) * p.sb_n, 0x7ffffffcu);
+    for (int i = 0; i < scales_a; i += 64) {
+      const int kb = (i + lane) / (MB * 16), row = (i + lane) % (MB * 16);
+      const uint32_t at = (uint32_t)min(row, (int)rows - 1) * (uint32_t)p.sa_row * 4u + (uint32_t)(kb0 + kb) * p.sa_block * 4u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)(sa_lds + i), 4, (int)(kb < kb_n ? at : F8B_NOWHERE), 0, 0, 0);
+    }
+    for (int i = 0; i < scales_b; i += 64)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, (lds_ptr_t)(sb_lds + i), 4, (int)(i + lane < kb_n ? (uint32_t)(kb0 + i + lane) * p.sb_block * 4u : F8B_NOWHERE), 0, 0, 0);
   };
   v4f acc[J][MB];
 #pragma unroll
@@ -151,6 +153,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
   int g = first;
   load_w(0, g);
   __builtin_amdgcn_sched_barrier(0);
+  load_scales();
+  __builtin_amdgcn_sched_barrier(0);
   load_act(g);
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (AHEAD == 1) {
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && MB * J >= 12 ? 1 : 2) void fp8_
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int u = w + i * NW, j = u / MB, mb = u - j * MB, n = n0 + j * 16 + q * 4, m = row0 + mb * 16 + r16;
-    if (u >= J * MB || n >= p.N || m >= p.M) continue;
+    if (u >= J * MB || n >= N || m >= M) continue;
     v4f val = red[u * 64 + lane];
 #pragma unroll
     for (int ww = 1; ww < NW; ++ww) val += red[(ww * (J * MB) + u) * 64 + lane];

@@ -25,6 +25,17 @@ struct QkArgs {
   int heads_q, heads_k, head_dim, rotary, lanes_log2;      // lanes: of a head
   float eps;
 };
+// What the first requests need arrives in registers with the launch: rows and positions, then the cache.
+__device__ inline int64_t join(uint32_t lo, uint32_t hi) { return (int64_t)((uint64_t)hi << 32 | lo); }
+inline v8u head_of_launch(const QkArgs& a) {
+  const uint64_t stride = (uint64_t)a.stride;
+  return v8u{ptr_lo(a.qkv), ptr_hi(a.qkv), ptr_lo(a.positions), ptr_hi(a.positions), (uint32_t)stride, (uint32_t)(stride >> 32),
+             (uint32_t)a.heads_q | (uint32_t)(a.head_dim / 8) << 20 | (uint32_t)a.lanes_log2 << 28, (uint32_t)a.heads_k};
+}
+inline v4u head2_of_launch(const QkArgs& a) {
+  const uint64_t stride = (uint64_t)a.cache_stride;
+  return v4u{ptr_lo(a.cache), ptr_hi(a.cache), (uint32_t)stride, (uint32_t)(stride >> 32)};
+}
 
 template <bool BF16>
 __device__ inline void unpack(v4u r, float (&f)[8]) {
@@ -69,52 +80,48 @@ __device__ inline void angles(const void* row, int at, float (&to)[8], int first
 }
 
 template <bool BF16, bool CACHE32, bool HALVES>
-__global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
+__global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const v8u head, const v4u head2, const QkArgs p) {
   using T = F16Traits<BF16>;
-  const int64_t token = blockIdx.x, position = p.positions[token];
+  const int heads_q = (int)(head[6] & 0xfffffu), heads_k = (int)head[7], head_dim = (int)(head[6] >> 20 & 0xffu) * 8, lanes_log2 = (int)(head[6] >> 28);
+  const int64_t token = blockIdx.x, position = head_ptr<int64_t>(head[2], head[3])[token];
+  __builtin_amdgcn_sched_barrier(0);      // (the first request: cos and sin wait for it)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int lanes = 1 << p.lanes_log2, per_wave = 64 >> p.lanes_log2;
+  const int lanes = 1 << lanes_log2, per_wave = 64 >> lanes_log2;
   const int e = (lane & (lanes - 1)) * 8;      // first of this lane's values in a head
-  const bool in_head = e < p.head_dim;
-  const int heads = p.heads_q + p.heads_k, rounds = (heads + per_wave - 1) / per_wave;
-  const uint16_t* const row = p.qkv + token * p.stride;
+  const bool in_head = e < head_dim;
+  const int heads = heads_q + heads_k, rounds = (heads + per_wave - 1) / per_wave;
+  const uint16_t* const row = head_ptr<uint16_t>(head[0], head[1]) + token * join(head[4], head[5]);
 
   v4u x[QK_AHEAD];
-  auto head_of = [&](int round) { return round * per_wave + (lane >> p.lanes_log2); };
+  auto head_of = [&](int round) { return round * per_wave + (lane >> lanes_log2); };
   auto request = [&](int first) {
 #pragma unroll
-    for (int i = 0; i < QK_AHEAD; ++i) {
-      const int h = head_of(first + i * (QK_T / 64));
-      x[i] = v4u{0u, 0u, 0u, 0u};
-      if (h < heads && in_head) x[i] = *reinterpret_cast<const v4u*>(row + (int64_t)h * p.head_dim + e);
-    }
+    for (int i = 0; i < QK_AHEAD; ++i)      // (without a branch: a lane behind the head or the heads reads the last one)
+      x[i] = *reinterpret_cast<const v4u*>(row + (int64_t)min(head_of(first + i * (QK_T / 64)), heads - 1) * head_dim + min(e, head_dim - 8));
   };
   int round = wave;
   request(round);      // (ahead of the wait for the position)
-  v4u raw_q = {0u, 0u, 0u, 0u}, raw_k = {0u, 0u, 0u, 0u};
-  if (in_head) {
-    raw_q = *reinterpret_cast<const v4u*>(p.q_weight + e);
-    raw_k = *reinterpret_cast<const v4u*>(p.k_weight + e);
-  }
-  if (position < 0 || position >= p.cache_rows) return;      // not a token of a sequence: its rows stay as they are
+  const v4u raw_q = *reinterpret_cast<const v4u*>(p.q_weight + min(e, head_dim - 8)), raw_k = *reinterpret_cast<const v4u*>(p.k_weight + min(e, head_dim - 8));
+  const bool written = position >= 0 && position < p.cache_rows;      // (or not a token of a sequence: its rows stay as they are.  A branch here would have the requests wait for it)
 
   // cos and sin of this lane's values; values that are not rotated have cos 1 and sin 0.  The second of a pair has + sin, the first - sin.
   float c[8], s[8], wq[8], wk[8];
   const int half = p.rotary / 2;
-  const void* const angle = (const char*)p.cache + position * p.cache_stride * (CACHE32 ? 4 : 2);
+  const void* const angle = head_ptr<char>(head2[0], head2[1]) + (written ? position : 0) * join(head2[2], head2[3]) * (CACHE32 ? 4 : 2);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     c[i] = 1.f;
     s[i] = 0.f;
   }
   if constexpr (HALVES) {
-    if (e < p.rotary) {      // (both halves are whole lanes)
-      const int at = e >= half ? e - half : e;
+    if (half > 0) {      // (both halves are whole lanes; a lane behind them reads the first one's)
+      const int at = e >= p.rotary ? 0 : e >= half ? e - half : e;
       angles<CACHE32, BF16, 8>(angle, at, c, 0);
       angles<CACHE32, BF16, 8>(angle, half + at, s, 0);
-      if (e < half) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = -s[i];
+      for (int i = 0; i < 8; ++i) {
+        c[i] = e < p.rotary ? c[i] : 1.f;
+        s[i] = e < half ? -s[i] : e < p.rotary ? s[i] : 0.f;
       }
     }
   } else {
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
   unpack<BF16>(raw_q, wq);
   unpack<BF16>(raw_k, wk);
   const int partner = !HALVES || e >= p.rotary ? lane : e < half ? lane + half / 8 : lane - half / 8;
-  const float over_dim = 1.0f / (float)p.head_dim;
+  const float over_dim = 1.0f / (float)head_dim;
 
   for (; round < rounds; round += QK_AHEAD * (QK_T / 64)) {
     if (round != wave) request(round);
@@ -150,9 +157,10 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
       unpack<BF16>(x[i], y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
-      const float rms = rsqrtf(group_sum(ss, p.lanes_log2) * over_dim + p.eps);
+      ss = in_head ? ss : 0.f;
+      const float rms = rsqrtf(group_sum(ss, lanes_log2) * over_dim + p.eps);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * rms * (h < p.heads_q ? wq[j] : wk[j]);
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * rms * (h < heads_q ? wq[j] : wk[j]);
       float z[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -160,11 +168,11 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
         z[j] = y[j] * c[j];
         if (e + j < p.rotary) z[j] += other * s[j];      // (a value that is not rotated stays what it is, whatever its neighbours are)
       }
-      if (h < heads && in_head) {
+      if (written && h < heads && in_head) {
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = (uint32_t)T::from_float(z[2 * j]) | (uint32_t)T::from_float(z[2 * j + 1]) << 16;
-        uint16_t* const to = h < p.heads_q ? p.q + (token * p.heads_q + h) * p.head_dim : p.k + (token * p.heads_k + h - p.heads_q) * p.head_dim;
+        uint16_t* const to = h < heads_q ? p.q + (token * heads_q + h) * head_dim : p.k + (token * heads_k + h - heads_q) * head_dim;
         *reinterpret_cast<v4u*>(to + e) = v4u{o[0], o[1], o[2], o[3]};
       }
     }
@@ -174,10 +182,10 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const QkArgs p) {
 template <bool BF16>
 void launch(const QkArgs& a, bool cache32, bool halves, int64_t tokens, hipStream_t s) {
   const dim3 grid((unsigned)tokens);
-  if (cache32 && halves) qk_norm_rope_kernel<BF16, true, true><<<grid, QK_T, 0, s>>>(a);
-  else if (cache32) qk_norm_rope_kernel<BF16, true, false><<<grid, QK_T, 0, s>>>(a);
-  else if (halves) qk_norm_rope_kernel<BF16, false, true><<<grid, QK_T, 0, s>>>(a);
-  else qk_norm_rope_kernel<BF16, false, false><<<grid, QK_T, 0, s>>>(a);
+  if (cache32 && halves) qk_norm_rope_kernel<BF16, true, true><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
+  else if (cache32) qk_norm_rope_kernel<BF16, true, false><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
+  else if (halves) qk_norm_rope_kernel<BF16, false, true><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
+  else qk_norm_rope_kernel<BF16, false, false><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
 }
 
 }  // namespace
@@ -205,6 +213,7 @@ extern "C" int vaq_qk_norm_rope(const void* qkv, int64_t qkv_row_stride, void* q
                 (long long)cos_sin_rows, (long long)cos_sin_row_stride);
   VAQ_CHECK_ARG((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_weight | (uintptr_t)k_weight) & 15) == 0 && (tokens == 1 || qkv_row_stride % 8 == 0),
                 "qk_norm_rope: rows and weights must be aligned to 16 bytes");
+  if (cos_sin_rows == 0) return VAQ_OK;      // every position lies outside
   QkArgs a{(const uint16_t*)qkv, (uint16_t*)q_out, (uint16_t*)k_out, (const uint16_t*)q_weight, (const uint16_t*)k_weight, cos_sin, positions, qkv_row_stride,
            cos_sin_row_stride, cos_sin_rows, (int)heads_q, (int)heads_k, (int)head_dim, (int)rotary_dim, 0, epsilon};
   while ((8 << a.lanes_log2) < head_dim) ++a.lanes_log2;
