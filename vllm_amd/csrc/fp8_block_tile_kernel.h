@@ -260,10 +260,22 @@ struct F8bOperandOffsets {
   }
 };
 
+// What the first requests need, which arrives in registers with the launch.
+struct F8bHead {
+  const uint8_t *a, *b;
+  uint32_t lda, ldb, tiles_m, tiles_n;
+  int K, M, N;
+};
+inline v8u f8b_head(const Fp8BlockParams& p) { return v8u{ptr_lo(p.a), ptr_hi(p.a), ptr_lo(p.b), ptr_hi(p.b), p.lda, p.ldb, (uint32_t)p.K, (uint32_t)p.M}; }
+inline v4u f8b_head2(const Fp8BlockParams& p, uint32_t tiles_m, uint32_t tiles_n) { return v4u{(uint32_t)p.N, tiles_m, tiles_n, 0u}; }
+__device__ inline F8bHead f8b_head_of(v8u h, v4u h2) {
+  return F8bHead{head_ptr<uint8_t>(h[0], h[1]), head_ptr<uint8_t>(h[2], h[3]), h[4], h[5], h2[1], h2[2], (int)h[6], (int)h[7], (int)h2[0]};
+}
+
 // BM x BN results through a ring of NST stages.  A step's fragments are in registers when it begins; its products run while the next step's fragments are read,
 // and its stage, which nobody needs any more, takes the operands NST steps on.  So NST - 1 steps are under way, and a step costs the longer of its LDS traffic and its products, and one
 // barrier.  The rows' scales travel with the operands (a load of four bytes a lane into the stage): loaded into registers a step ahead they would be answered behind
-// the operands of all steps under way, which the wait for them would then be a wait for.  The columns' scales of all of K are requested once, ahead of everything.
+// the operands of all steps under way, which the wait for them would then be a wait for.  The columns' scales of all of K are requested once, behind the first step's operands.
 template <int BM, int BN, int NST>
 struct F8bRing {
   static constexpr int SCALES = BM * 128 + BN * 128, STAGE = SCALES + BM * 4;
@@ -271,7 +283,7 @@ struct F8bRing {
   __host__ __device__ static inline int sb_floats(int K) { return ((K + F8B - 1) / F8B + 1 + 63) / 64 * 64; }      // of a block of columns: one past K, which is zero
 };
 template <bool BF16, int BM, int BN, int WAVES_M, int WAVES_N, int NST, bool TAIL>
-__global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
+__global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kernel(const v8u head, const v4u head2, const Fp8BlockParams p) {
   constexpr int NW = WAVES_M * WAVES_N, TM = BM / WAVES_M, TN = BN / WAVES_N;
   using Wave = F8bWave<BF16, TM, TN>;
   using Ring = F8bRing<BM, BN, NST>;
@@ -279,37 +291,38 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   static_assert(BM <= 64 * NW, "each wavefront asks for the scales of 64 rows");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WAVES_N, wn = wave % WAVES_N;
-  const uint32_t position = f8b_position(blockIdx.x, tiles_m * tiles_n);
-  if (position >= tiles_m * tiles_n) return;
-  const F8bTile tile = f8b_tile(position, tiles_m, tiles_n, BM, BN);
-  const int m0 = tile.m0, n0 = tile.n0, rows = min(BM, p.M - m0), steps = (p.K + F8B - 1) / F8B;
+  const F8bHead h = f8b_head_of(head, head2);
+  const uint32_t position = f8b_position(blockIdx.x, h.tiles_m * h.tiles_n);
+  if (position >= h.tiles_m * h.tiles_n) return;
+  const F8bTile tile = f8b_tile(position, h.tiles_m, h.tiles_n, BM, BN);
+  const int m0 = tile.m0, n0 = tile.n0, rows = min(BM, h.M - m0), steps = (h.K + F8B - 1) / F8B;
   F8bOperandOffsets<BM, NW, TAIL> a;
   F8bOperandOffsets<BN, NW, TAIL> b;
-  a.start(p.a, m0, rows, p.lda, p.K, wave);
-  b.start(p.b, n0, min(BN, p.N - n0), p.ldb, p.K, wave);
+  a.start(h.a, m0, rows, h.lda, h.K, wave);
+  b.start(h.b, n0, min(BN, h.N - n0), h.ldb, h.K, wave);
   Wave w;
   w.start();
   typedef __attribute__((address_space(3))) void* lds_ptr_t;
-  const int sb_floats = Ring::sb_floats(p.K);
+  const int sb_floats = Ring::sb_floats(h.K);
   float* const sb_lds = reinterpret_cast<float*>(lds8 + NST * Ring::STAGE);      // [block of columns][block of K]
-  {
+  auto request_columns_scales = [&] {
     // (every wavefront asks for all of them: each then waits for its own requests only)
-    const int nb0 = n0 / F8B, nb_n = (p.N + F8B - 1) / F8B - nb0;
+    const int nb0 = n0 / F8B, nb_n = (h.N + F8B - 1) / F8B - nb0;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
       for (int i = 0; i < sb_floats; i += 64)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sb + (int64_t)(nb0 + (nb < nb_n ? nb : 0)) * p.sb_n, 0x7ffffffcu), (lds_ptr_t)(sb_lds + nb * sb_floats + i), 4,
                                                  (int)(i + lane < steps ? (uint32_t)(i + lane) * p.sb_block * 4u : F8B_NOWHERE), 0, 0, 0);
-  }
+  };
   const int sa_first = wave % (BM / 64) * 64;
   const uint32_t vsa = (uint32_t)min(sa_first + lane, rows - 1) * (uint32_t)p.sa_row * 4u, sa_step = p.sa_block * 4u;
   uint32_t k = 0, sa_next = 0;      // the block that is requested next; past K: nothing
   auto request = [&](uint8_t* at) {
-    const bool some = k < (uint32_t)p.K;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, some ? 0x7ffffffcu : 0u), (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)vsa,
-                                             (int)(some ? sa_next : 0u), 0, 0);
+    const bool some = k < (uint32_t)h.K;
     a.request(k, at);
     b.request(k, at + BM * 128);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(f8b_rsrc(p.sa + (int64_t)m0 * p.sa_row, some ? 0x7ffffffcu : 0u), (lds_ptr_t)(at + Ring::SCALES + sa_first * 4), 4, (int)vsa,
+                                             (int)(some ? sa_next : 0u), 0, 0);
     k += F8B;
     sa_next += sa_step;
   };
@@ -334,8 +347,12 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
   // Behind a step's operands come those of the next NST - 2 steps.
   constexpr int OPS = a.LD + b.LD + 1;
   static_assert((NST - 1) * OPS <= 63, "wait counter range");
+  request(lds8);
+  __builtin_amdgcn_sched_barrier(0);
+  request_columns_scales();
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int s = 0; s < NST; ++s) request(lds8 + s * Ring::STAGE);
+  for (int s = 1; s < NST; ++s) request(lds8 + s * Ring::STAGE);
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NST - 1) * OPS) : "memory");
   Step even, odd;
   int stage = 0;      // in bytes
@@ -372,34 +389,37 @@ __global__ __launch_bounds__(WAVES_M * WAVES_N * 64, 2) void fp8_block_tile_kern
 // A step of a wavefront is [read columns and rows 0 .. 31, request B(s + 2)] barrier [products of rows 0 .. 63, read rows 32 .. 95] barrier [read rows 96 .. 127, request A(s + 2),
 // wait for what step s + 1 reads] barrier [products of rows 64 .. 127] barrier; the late half of the workgroup passes one extra barrier first and skips its last one, so that every wavefront passes the same number.
 template <bool BF16, bool TAIL>
-__global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const Fp8BlockParams p, const uint32_t tiles_m, const uint32_t tiles_n) {
+__global__ __launch_bounds__(512) void fp8_block_tile256_kernel(const v8u head, const v4u head2, const Fp8BlockParams p) {
   constexpr int B = 256, NW = 8, TM = 128, TN = 64, PLACE = B * 128;
   using Wave = F8bWaveScales<BF16, TM, TN>;
   constexpr int NT = Wave::NT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
   const bool late = wave >= 4;      // wavefronts w and w + 4 share a SIMD
-  const uint32_t position = f8b_position(blockIdx.x, tiles_m * tiles_n);
-  if (position >= tiles_m * tiles_n) return;
-  const F8bTile tile = f8b_tile(position, tiles_m, tiles_n, B, B);
-  const int m0 = tile.m0, n0 = tile.n0, rows = min(B, p.M - m0);
+  const F8bHead h = f8b_head_of(head, head2);
+  const uint32_t position = f8b_position(blockIdx.x, h.tiles_m * h.tiles_n);
+  if (position >= h.tiles_m * h.tiles_n) return;
+  const F8bTile tile = f8b_tile(position, h.tiles_m, h.tiles_n, B, B);
+  const int m0 = tile.m0, n0 = tile.n0, rows = min(B, h.M - m0);
 
   F8bOperand<B, NW, TAIL> a, b;
-  a.start(p.a, m0, rows, p.lda, p.K, wave);
-  b.start(p.b, n0, min(B, p.N - n0), p.ldb, p.K, wave);
-  Wave w;
-  w.start(p, m0, wm * TM, rows, n0 + wn * TN, n0);
+  a.start(h.a, m0, rows, h.lda, h.K, wave);
+  b.start(h.b, n0, min(B, h.N - n0), h.ldb, h.K, wave);
   constexpr int LD = a.LD;      // requests of a wavefront for an operand
 
-  const int steps = (p.K + F8B - 1) / F8B;
+  const int steps = (h.K + F8B - 1) / F8B;
   int qb = 0;      // place of this step's weights
   auto place = [&](int ahead) {
     const int q = qb + ahead;
     return lds8 + (q >= 5 ? q - 5 : q) * PLACE;
   };
-  typename Wave::Scales first = w.request_scales(0), now = w.request_scales((uint32_t)min(1, steps - 1));
   b.request(0, place(0));
   a.request(0, place(1));
+  __builtin_amdgcn_sched_barrier(0);      // (what follows waits for arguments)
+  Wave w;
+  w.start(p, m0, wm * TM, rows, n0 + wn * TN, n0);
+  typename Wave::Scales first = w.request_scales(0), now = w.request_scales((uint32_t)min(1, steps - 1));
+  __builtin_amdgcn_sched_barrier(0);
   b.request(F8B, place(2));
   a.request(F8B, place(3));
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LD) : "memory");
