@@ -9,7 +9,8 @@ template <int BM, int BN, int WAVES, typename Kernel>
 static int launch_tiles(const Fp8BlockParams& p, size_t lds, Kernel kern, size_t (&reserved)[VAQ_MAX_DEVICES], hipStream_t s) {
   const uint32_t tiles_m = ((uint32_t)p.M + BM - 1) / BM, tiles_n = ((uint32_t)p.N + BN - 1) / BN;
   if (const int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), lds, reserved, "fp8_block_scaled_mm"); rc != VAQ_OK) return rc;
-  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), lds, s, f8b_head(p), f8b_head2(p, tiles_m, tiles_n), p);
+  const KernelHead h = f8b_head(p, tiles_m, tiles_n);
+  hipLaunchKernelGGL(kern, dim3((tiles_m * tiles_n + 7) / 8 * 8), dim3(WAVES * 64), lds, s, h.a, h.b, p);
   return VAQ_OK;
 }
 // tile shapes: rows, columns, wavefronts along both, stages of the ring

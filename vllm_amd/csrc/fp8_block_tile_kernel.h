@@ -266,8 +266,9 @@ struct F8bHead {
   uint32_t lda, ldb, tiles_m, tiles_n;
   int K, M, N;
 };
-inline v8u f8b_head(const Fp8BlockParams& p) { return v8u{ptr_lo(p.a), ptr_hi(p.a), ptr_lo(p.b), ptr_hi(p.b), p.lda, p.ldb, (uint32_t)p.K, (uint32_t)p.M}; }
-inline v4u f8b_head2(const Fp8BlockParams& p, uint32_t tiles_m, uint32_t tiles_n) { return v4u{(uint32_t)p.N, tiles_m, tiles_n, 0u}; }
+inline KernelHead f8b_head(const Fp8BlockParams& p, uint32_t tiles_m, uint32_t tiles_n) {
+  return KernelHead{v8u{ptr_lo(p.a), ptr_hi(p.a), ptr_lo(p.b), ptr_hi(p.b), p.lda, p.ldb, (uint32_t)p.K, (uint32_t)p.M}, v4u{(uint32_t)p.N, tiles_m, tiles_n, 0u}, v2u{}};
+}
 __device__ inline F8bHead f8b_head_of(v8u h, v4u h2) {
   return F8bHead{head_ptr<uint8_t>(h[0], h[1]), head_ptr<uint8_t>(h[2], h[3]), h[4], h[5], h2[1], h2[2], (int)h[6], (int)h[7], (int)h2[0]};
 }

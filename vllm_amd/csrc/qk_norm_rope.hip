@@ -27,14 +27,11 @@ struct QkArgs {
 };
 // What the first requests need arrives in registers with the launch: rows and positions, then the cache.
 __device__ inline int64_t join(uint32_t lo, uint32_t hi) { return (int64_t)((uint64_t)hi << 32 | lo); }
-inline v8u head_of_launch(const QkArgs& a) {
-  const uint64_t stride = (uint64_t)a.stride;
-  return v8u{ptr_lo(a.qkv), ptr_hi(a.qkv), ptr_lo(a.positions), ptr_hi(a.positions), (uint32_t)stride, (uint32_t)(stride >> 32),
-             (uint32_t)a.heads_q | (uint32_t)(a.head_dim / 8) << 20 | (uint32_t)a.lanes_log2 << 28, (uint32_t)a.heads_k};
-}
-inline v4u head2_of_launch(const QkArgs& a) {
-  const uint64_t stride = (uint64_t)a.cache_stride;
-  return v4u{ptr_lo(a.cache), ptr_hi(a.cache), (uint32_t)stride, (uint32_t)(stride >> 32)};
+inline KernelHead head_of_launch(const QkArgs& a) {
+  const uint64_t stride = (uint64_t)a.stride, cache_stride = (uint64_t)a.cache_stride;
+  return KernelHead{v8u{ptr_lo(a.qkv), ptr_hi(a.qkv), ptr_lo(a.positions), ptr_hi(a.positions), (uint32_t)stride, (uint32_t)(stride >> 32),
+                        (uint32_t)a.heads_q | (uint32_t)(a.head_dim / 8) << 20 | (uint32_t)a.lanes_log2 << 28, (uint32_t)a.heads_k},
+                    v4u{ptr_lo(a.cache), ptr_hi(a.cache), (uint32_t)cache_stride, (uint32_t)(cache_stride >> 32)}, v2u{}};
 }
 
 template <bool BF16>
@@ -182,10 +179,11 @@ __global__ __launch_bounds__(QK_T) void qk_norm_rope_kernel(const v8u head, cons
 template <bool BF16>
 void launch(const QkArgs& a, bool cache32, bool halves, int64_t tokens, hipStream_t s) {
   const dim3 grid((unsigned)tokens);
-  if (cache32 && halves) qk_norm_rope_kernel<BF16, true, true><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
-  else if (cache32) qk_norm_rope_kernel<BF16, true, false><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
-  else if (halves) qk_norm_rope_kernel<BF16, false, true><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
-  else qk_norm_rope_kernel<BF16, false, false><<<grid, QK_T, 0, s>>>(head_of_launch(a), head2_of_launch(a), a);
+  const KernelHead h = head_of_launch(a);
+  if (cache32 && halves) qk_norm_rope_kernel<BF16, true, true><<<grid, QK_T, 0, s>>>(h.a, h.b, a);
+  else if (cache32) qk_norm_rope_kernel<BF16, true, false><<<grid, QK_T, 0, s>>>(h.a, h.b, a);
+  else if (halves) qk_norm_rope_kernel<BF16, false, true><<<grid, QK_T, 0, s>>>(h.a, h.b, a);
+  else qk_norm_rope_kernel<BF16, false, false><<<grid, QK_T, 0, s>>>(h.a, h.b, a);
 }
 
 }  // namespace
