@@ -153,3 +153,23 @@ def test_linear_of_the_last_token_of_each_sequence(device):
     got = ops.block_fp8_linear(x[:, -1:], w, sw, torch.bfloat16, None)
     assert got.shape == (3, 1, 144)
     assert torch.equal(got, ops.block_fp8_linear(x[:, -1:].contiguous(), w, sw, torch.bfloat16, None))
+
+
+def test_two_results_of_a_call_lie_apart(device):
+    """They may be one allocation: each is a whole tensor of its own all the same."""
+    from vllm_amd import _custom_ops as ops
+    x = torch.randn((3, 260), device=device).to(torch.bfloat16)
+    qkv, head = torch.randn((3, 5 * 24), device=device).to(torch.bfloat16), torch.ones(24, device=device, dtype=torch.bfloat16)
+    pairs = [ops.scaled_fp8_group_quant(x), ops.silu_and_mul_group_quant(x), ops.rms_norm_group_quant(x, x[0], 1e-5),
+             ops.qk_norm_rope(qkv, 3, 2, 24, 1e-6, head, head, torch.ones((4, 16), device=device), torch.tensor([0, 3, 1], device=device))]
+    for a, b in pairs:
+        assert a.is_contiguous() and not a.requires_grad and not b.requires_grad and a._version == 0 and b._version == 0
+        one, other = a.clone(), b.clone()
+        b.zero_()
+        assert torch.equal(a.view(torch.uint8), one.view(torch.uint8)) and bool((b == 0).all()) and a._version == 0
+        b.copy_(other)
+        a.view(torch.uint8).zero_()
+        assert torch.equal(b, other)
+        kept = b
+        del a, b
+        assert torch.equal(kept, other)

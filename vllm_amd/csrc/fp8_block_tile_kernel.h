@@ -2,8 +2,14 @@
 //
 //  * BM x BN results a workgroup; a step is one block of K.  Both operands come by direct-to-LDS loads of whole 128-byte lines (8 rows an instruction) into a
 //    ring of NST stages; chunk c of a row lies at place c ^ (row / 2 & 7) of its 128 bytes, so that the 16 lanes that are served together hit all banks.
-//  * The products of 16 rows are issued ahead of the multiply-adds of the 16 rows before them, which then find their results ready: four multiply-adds go beside an
-//    instruction that keeps the matrix core for 32 cycles.
+//  * A product is issued behind the four multiply-adds that add the one before it in its registers: they find their result ready, and run beside an instruction
+//    that keeps the matrix core for 32 cycles (measured without a loss of the product's rate).
+//
+// 4096 x 4096 x 28672: 404 .. 422 us by 256 x 256 tiles = 2.3 PFLOP/s, the rate of the library's 8192^3 product without block scales (2.25 .. 2.31), and the card's power limit
+// (zeros run a quarter faster).  333 rows, K = 2976, N = 10240: 18.6 us by 128 x 128 tiles on 240 of 256 compute units, 24 with cold weights; bytes 7.5, products 9.
+// What bounds the smaller tiles is LDS traffic: a step of a 128 x 128 tile is 98 KB read and 33 KB written, 1020 cycles of LDS, 512 of products, 1150 measured.  Tried
+// without a gain: four wavefronts of 64 x 64 (less traffic, nothing to run beside it: 3 % either way), two blocks of K a step, fewer stages and two workgroups on a compute
+// unit (3 % .. 2 x slower where there is one tile a compute unit), weights from memory straight into registers (1.0 .. 1.7 x the time).
 #pragma once
 #include "fp8_block_mm.h"
 
