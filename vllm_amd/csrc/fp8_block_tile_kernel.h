@@ -9,7 +9,7 @@
 // (zeros run a quarter faster).  333 rows, K = 2976, N = 10240: 18.6 us by 128 x 128 tiles on 240 of 256 compute units, 24 with cold weights; bytes 7.5, products 9.
 // What bounds the smaller tiles is LDS traffic: a step of a 128 x 128 tile is 98 KB read and 33 KB written, 1020 cycles of LDS, 512 of products, 1150 measured.  Tried
 // without a gain: four wavefronts of 64 x 64 (less traffic, nothing to run beside it: 3 % either way), two blocks of K a step, fewer stages and two workgroups on a compute
-// unit (3 % .. 2 x slower where there is one tile a compute unit), weights from memory straight into registers (1.0 .. 1.7 x the time).
+// unit (8 .. 60 % slower where there is one tile a compute unit), weights from memory straight into registers (1.0 .. 1.3 x the time).
 #pragma once
 #include "fp8_block_mm.h"
 
