@@ -173,3 +173,17 @@ def test_two_results_of_a_call_lie_apart(device):
         kept = b
         del a, b
         assert torch.equal(kept, other)
+
+
+def test_results_in_inference_mode_and_without_gradients(device):
+    from vllm_amd import _custom_ops as ops
+    x, w = torch.randn((5, 256), device=device).to(torch.bfloat16), (torch.randn((128, 256), device=device) * 40).to(FP8).t()
+    sw = torch.rand((2, 1), device=device)
+    want, scales = ops.scaled_fp8_group_quant(x)
+    product = ops.block_scaled_mm(want, w, scales, sw, torch.bfloat16)
+    for mode in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        with mode():
+            codes, s = ops.scaled_fp8_group_quant(x)
+            assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(s, scales) and codes.is_inference() == s.is_inference()
+            assert torch.equal(ops.block_scaled_mm(codes, w, s, sw, torch.bfloat16), product)
+            assert torch.equal(s.clone().mul_(2), scales * 2)

@@ -48,22 +48,22 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStre
 // ----------------------------------------------------------------------------- choice of the kernel
 // The cheapest plan by price, in us.  Rows: a step is a latency, the bytes into the compute unit or the products, whichever is longest; a workgroup is its start, its steps and its
 // meeting; beside all of them the weights from memory, once and a share for every further block of rows.  Tiles: rounds of workgroups (a last, partly filled one costs a share of
-// a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 9891
-// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 2967 that the fit had not seen the cheapest plan takes 1.013 of the fastest one's time
-// in the mean; without eight wavefronts 1.019, without any one of the tile shapes 1.016 .. 1.027.  (profiles/plan_prices/fp8_block.py)
+// a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 6556
+// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 2998 that the fit had not seen the cheapest plan takes 1.010 of the fastest one's time
+// in the mean; without eight wavefronts 1.018, without any one of the tile shapes 1.013 .. 1.032.  (profiles/plan_prices/fp8_block.py)
 constexpr double ROWS_PRICE[4][9] = {      // by steps ahead and wavefronts: 1, 4; 1, 8; 2, 4; 2, 8
-    {0.7175, 0.2233, 0.08537, 0.5477, 0.1458, 0.2031, 0.3329, 1.852, 1.326e-07},
-    {0.6447, 0.1456, 0.2614, 0.8933, 2.161e-09, 0.2047, 0.4566, 1.853, 0.6736},
-    {0.4789, 0.2017, 0.1329, 1.073, 0.07598, 0.21, 0.3385, 1.632, 0.3615},
-    {0.1219, 0.1974, 0.01679, 1.342, 5.481e-09, 0.2228, 0.4273, 1.603, 0.5403},
+    {0.701, 0.2198, 0.08786, 0.374, 0.1317, 0.2013, 0.3504, 1.73, 2.986e-07},
+    {0.6413, 0.1219, 0.2373, 0.8801, 1.031e-08, 0.2089, 0.458, 1.845, 0.6726},
+    {0.4638, 0.2044, 0.1229, 0.8819, 0.0671, 0.2038, 0.3379, 1.506, 0.3787},
+    {0.1988, 0.1996, 0.08961, 1.077, 1.163e-08, 0.2129, 0.4428, 1.479, 0.3934},
 };
 constexpr double TILE_PRICE[F8B_SHAPES][8] = {
-    {0.801, 2.021, 0.2395, 0.2008, 0.2297, 2.067, 0.4606, 0.1698},
-    {0.8389, 1.406, 0.3627, 0.2204, 0.1846, 2.792, 0.79, 0.2233},
-    {0.7977, 2.238, 0.5305, 0.2131, 0.1959, 2.736, 0.334, 0.1353},
-    {0.7573, 2.982, 0.8615, 0.2674, 0.02411, 3.191, 0.2571, 0.1805},
-    {0.7526, 4.047, 0.8291, 0.1418, 1.137e-06, 2.734, 0.1566, 0.08221},
-    {0.816, 5.459, 1.417, 0.2169, 0.2788, 2.903, 0.1247, 0.05883},
+    {0.8083, 2.155, 0.2425, 0.1994, 0.3173, 1.605, 0.2106, 0.124},
+    {0.7579, 2.032, 0.3918, 0.2017, 0.1988, 2.113, 0.3888, 0.2262},
+    {0.7247, 3.037, 0.577, 0.1987, 0.2703, 1.9, 0.1331, 0.1242},
+    {0.7072, 4.343, 0.9214, 0.2349, 0.09186, 1.979, 0.2059, 0.1603},
+    {0.7522, 4.584, 0.8417, 0.173, 0.834, 1.697, 0.1879, 0.08089},
+    {0.7887, 5.882, 1.463, 0.2048, 0.6666, 2.231, 0.1658, 0.05556},
 };
 constexpr int TILE_ROWS[F8B_SHAPES] = {64, 64, 128, 128, 256, 256}, TILE_COLUMNS[F8B_SHAPES] = {64, 128, 128, 256, 128, 256};
 static double cubes(double a, double b, double c = 0) { return cbrt(a * a * a + b * b * b + c * c * c); }
