@@ -7,9 +7,10 @@
 //
 // 4096 x 4096 x 28672: 404 .. 422 us by 256 x 256 tiles = 2.3 PFLOP/s, the rate of the library's 8192^3 product without block scales (2.25 .. 2.31), and the card's power limit
 // (zeros run a quarter faster).  333 rows, K = 2976, N = 10240: 18.6 us by 128 x 128 tiles on 240 of 256 compute units, 24 with cold weights; bytes 7.5, products 9.
-// What bounds the smaller tiles is LDS traffic: a step of a 128 x 128 tile is 98 KB read and 33 KB written, 1020 cycles of LDS, 512 of products, 1150 measured.  Tried
-// without a gain: four wavefronts of 64 x 64 (less traffic, nothing to run beside it: 3 % either way), two blocks of K a step, fewer stages and two workgroups on a compute
-// unit (8 .. 60 % slower where there is one tile a compute unit), weights from memory straight into registers (1.0 .. 1.3 x the time).
+// What bounds the smaller tiles is the operands' way into a compute unit: 790 KB in 17 us there, 46 .. 53 bytes/ns on all shapes timed, cold (a probe that only reads
+// gets 47 cold, 76 from the last-level cache, 115 from the L2).  So more wavefronts do not help: two groups of four with half of K each on a compute unit take the same
+// time (12.6 us at 128 x 4096 x 4096), and neither does less LDS traffic: four wavefronts of 64 x 64 (3 % either way), weights from memory straight into registers
+// (1.0 .. 1.3 x the time).  Nor two blocks of K a step (level), or fewer stages and two workgroups on a compute unit (8 .. 60 % slower where there is one tile for each).
 #pragma once
 #include "fp8_block_mm.h"
 
