@@ -16,7 +16,7 @@ import numpy as np
 
 HERE = Path(__file__).resolve().parent
 SOURCE = HERE.parent.parent / "vllm_amd" / "csrc" / "fp8_block_mm.hip"
-CUS, SHAPES = 256, [(64, 64), (64, 128), (128, 128), (128, 256), (256, 128), (256, 256)]
+CUS, SHAPES = 256, [(64, 64), (64, 128), (128, 128), (128, 256), (256, 128), (256, 256), (128, 64)]
 
 
 def tables() -> tuple[dict, list]:

@@ -232,7 +232,7 @@ def test_prices_are_those_of_the_fit_and_choose_well():
     f = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(f)
     few, tiles = f.tables()
-    assert [len(r) for r in few.values()] == [9] * 4 and [len(r) for r in tiles] == [8] * 6
+    assert [len(r) for r in few.values()] == [9] * 4 and [len(r) for r in tiles] == [8] * 7
     _, by_problem = f.load()
     problems = list(by_problem)[:300]
     assert f.choice({p: by_problem[p] for p in problems}, few, tiles).mean() < 1.03
@@ -255,4 +255,4 @@ def test_every_plan_in_reach_is_built():
             for n in (16, 144, 4096, 28672, 262144):
                 assert lib.vaq_fp8_block_plan(m, n, k, plan) == 0 and plan[5] > 0
                 mb, j, ahead, waves, shape = map(int, plan[:5])
-                assert (mb == 0 and 0 <= shape < 6) or ((mb + ahead * j) * waves < 40 and j in (1, 2, 4) and (waves == 4 or j == 1) and (j < 4 or ahead == 1))
+                assert (mb == 0 and 0 <= shape < 7) or ((mb + ahead * j) * waves < 40 and j in (1, 2, 4) and (waves == 4 or j == 1) and (j < 4 or ahead == 1))

@@ -9,7 +9,7 @@ from oracle import fp8_block as ob
 pytestmark = pytest.mark.gpu
 
 FP8 = torch.float8_e4m3fn
-SHAPES = 6      # tile shapes
+SHAPES = 7      # tile shapes
 # blocks of 16 rows, n-tiles, steps ahead, wavefronts
 ROWS = [(mb, j, ahead, waves) for mb in (1, 2, 3, 4) for j in (1, 2, 4) for ahead in (1, 2) for waves in (4, 8)
         if (mb + ahead * j) * waves < 40 and (waves == 4 or j == 1) and (j < 4 or ahead == 1)]

@@ -43,7 +43,7 @@ size_t fp8_block_rows_lds_bytes(int64_t K, const F8bRows& r);
 bool fp8_block_rows_fits(int64_t K, const F8bRows& r);
 bool fp8_block_rows_launch(const Fp8BlockParams& p, bool bf16, const F8bRows& r, hipStream_t s);
 // tiles (fp8_block_tile_kernel.h)
-constexpr int F8B_SHAPES = 6;
+constexpr int F8B_SHAPES = 7;
 int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStream_t s);
 
 }  // namespace vaq

@@ -38,6 +38,7 @@ static int launch_type(const Fp8BlockParams& p, int shape, hipStream_t s) {
     case 2: return launch_shape<BF16, 128, 128, 2, 4, 4>(p, s);
     case 3: return launch_shape<BF16, 128, 256, 2, 4, 3>(p, s);
     case 4: return launch_shape<BF16, 256, 128, 4, 2, 3>(p, s);
+    case 6: return launch_shape<BF16, 128, 64, 4, 2, 6>(p, s);
     default: return launch_256<BF16>(p, s);
   }
 }
@@ -48,24 +49,25 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStre
 // ----------------------------------------------------------------------------- choice of the kernel
 // The cheapest plan by price, in us.  Rows: a step is a latency, the bytes into the compute unit or the products, whichever is longest; a workgroup is its start, its steps and its
 // meeting; beside all of them the weights from memory, once and a share for every further block of rows.  Tiles: rounds of workgroups (a last, partly filled one costs a share of
-// a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 6556
-// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 2998 that the fit had not seen the cheapest plan takes 1.010 of the fastest one's time
-// in the mean; without eight wavefronts 1.018, without any one of the tile shapes 1.013 .. 1.032.  (profiles/plan_prices/fp8_block.py)
+// a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 4031
+// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 1730 that the fit had not seen the cheapest plan takes 1.011 of the fastest one's time
+// in the mean; without eight wavefronts 1.018, without any one of the tile shapes 1.012 .. 1.033.  (profiles/plan_prices/fp8_block.py)
 constexpr double ROWS_PRICE[4][9] = {      // by steps ahead and wavefronts: 1, 4; 1, 8; 2, 4; 2, 8
-    {0.701, 0.2198, 0.08786, 0.374, 0.1317, 0.2013, 0.3504, 1.73, 2.986e-07},
-    {0.6413, 0.1219, 0.2373, 0.8801, 1.031e-08, 0.2089, 0.458, 1.845, 0.6726},
-    {0.4638, 0.2044, 0.1229, 0.8819, 0.0671, 0.2038, 0.3379, 1.506, 0.3787},
-    {0.1988, 0.1996, 0.08961, 1.077, 1.163e-08, 0.2129, 0.4428, 1.479, 0.3934},
+    {0.7038, 0.217, 0.08696, 0.3525, 0.1332, 0.1972, 0.3488, 1.744, 8.075e-08},
+    {0.6413, 0.1219, 0.2373, 0.8801, 3.759e-09, 0.2089, 0.458, 1.845, 0.6726},
+    {0.4628, 0.2024, 0.123, 0.8821, 0.06831, 0.2003, 0.3304, 1.504, 0.3148},
+    {0.1983, 0.1981, 0.09101, 1.083, 6.719e-09, 0.2081, 0.4423, 1.482, 0.3933},
 };
 constexpr double TILE_PRICE[F8B_SHAPES][8] = {
-    {0.8083, 2.155, 0.2425, 0.1994, 0.3173, 1.605, 0.2106, 0.124},
-    {0.7579, 2.032, 0.3918, 0.2017, 0.1988, 2.113, 0.3888, 0.2262},
-    {0.7247, 3.037, 0.577, 0.1987, 0.2703, 1.9, 0.1331, 0.1242},
-    {0.7072, 4.343, 0.9214, 0.2349, 0.09186, 1.979, 0.2059, 0.1603},
-    {0.7522, 4.584, 0.8417, 0.173, 0.834, 1.697, 0.1879, 0.08089},
-    {0.7887, 5.882, 1.463, 0.2048, 0.6666, 2.231, 0.1658, 0.05556},
+    {0.8069, 2.116, 0.2367, 0.1964, 0.3056, 1.63, 0.2593, 0.1684},
+    {0.7361, 1.904, 0.3832, 0.1829, 0.2016, 2.272, 0.4499, 0.301},
+    {0.743, 2.82, 0.5552, 0.1841, 0.2579, 2.002, 0.1814, 0.1479},
+    {0.7305, 4.074, 0.8848, 0.2526, 0.09163, 2.121, 0.2139, 0.1661},
+    {0.771, 4.56, 0.8191, 0.1713, 0.7118, 1.68, 0.183, 0.07507},
+    {0.8033, 5.69, 1.438, 0.1896, 0.57, 2.301, 0.1616, 0.05301},
+    {0.7719, 2.926, 0.364, 0.1916, 0.3317, 1.662, 0.1059, 0.1476},
 };
-constexpr int TILE_ROWS[F8B_SHAPES] = {64, 64, 128, 128, 256, 256}, TILE_COLUMNS[F8B_SHAPES] = {64, 128, 128, 256, 128, 256};
+constexpr int TILE_ROWS[F8B_SHAPES] = {64, 64, 128, 128, 256, 256, 128}, TILE_COLUMNS[F8B_SHAPES] = {64, 128, 128, 256, 128, 256, 64};
 static double cubes(double a, double b, double c = 0) { return cbrt(a * a * a + b * b * b + c * c * c); }
 
 static double rows_us(const F8bRows& r, double M, double N, double K, int cus) {

@@ -9,7 +9,7 @@
 // (zeros run a quarter faster).  333 rows, K = 2976, N = 10240: 18.6 us by 128 x 128 tiles on 240 of 256 compute units, 24 with cold weights; bytes 7.5, products 9.
 // What bounds the smaller tiles is the operands' way into a compute unit: 790 KB in 17 us there, 46 .. 53 bytes/ns on all shapes timed, cold (a probe that only reads
 // gets 47 cold, 76 from the last-level cache, 115 from the L2).  So more wavefronts do not help: two groups of four with half of K each on a compute unit take the same
-// time (12.6 us at 128 x 4096 x 4096), and neither does less LDS traffic: four wavefronts of 64 x 64 (3 % either way), weights from memory straight into registers
+// time (12.6 us at 128 x 4096 x 4096, 64 x 64 tiles), and neither does less LDS traffic: four wavefronts of 64 x 64 (3 % either way), weights from memory straight into registers
 // (1.0 .. 1.3 x the time).  Nor two blocks of K a step (level), or fewer stages and two workgroups on a compute unit (8 .. 60 % slower where there is one tile for each).
 #pragma once
 #include "fp8_block_mm.h"
@@ -113,6 +113,7 @@ struct F8bWave {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();      // lanes exchange data through LDS; its operations run in program order
         constexpr int CHUNKS = TN / 8;        // of 16 bytes in a row
+        static_assert(16 * CHUNKS % 64 == 0, "whole wavefronts");
 #pragma unroll
         for (int c = 0; c < 16 * CHUNKS; c += 64) {
           const int row = (c + lane) / CHUNKS, chunk = (c + lane) % CHUNKS;
