@@ -286,7 +286,7 @@ int vaq_rms_norm_fp8_group_quant(uint8_t* out, float* scales, int64_t scale_row_
  *   sa    fp32, that of row m and block kb at sa[m * sa_row_stride + kb * sa_block_stride]
  *   sb    fp32, that of block kb of K and nb of N at sb[kb * sb_k_stride + nb * sb_n_stride]
  *   bias  [N] of the type of out or NULL;  out [M, N] F16 / BF16, 8-byte aligned, row stride ldc elements (a multiple of 4)
- * K and N are multiples of 16; their last blocks may be shorter than 128.  No scratch.
+ * K and N are multiples of 16; their last blocks may be shorter than 128.  With M = 1 lda, ldc and sa_row_stride are not looked at.  No scratch.
  */
 int vaq_fp8_block_scaled_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb, const float* sa, int64_t sa_row_stride,
                             int64_t sa_block_stride, const float* sb, int64_t sb_k_stride, int64_t sb_n_stride, const void* bias, void* out,

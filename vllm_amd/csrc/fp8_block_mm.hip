@@ -173,11 +173,15 @@ extern "C" int vaq_fp8_block_scaled_mm_tuned(const uint8_t* a, int64_t lda, cons
   VAQ_CHECK_ARG(a && b && sa && sb && out, "fp8_block_scaled_mm: null pointer");
   VAQ_CHECK_ARG((((uintptr_t)a | (uintptr_t)b) & 15) == 0 && ((uintptr_t)out & 7) == 0 && (((uintptr_t)sa | (uintptr_t)sb) & 3) == 0 && ((uintptr_t)bias & 1) == 0,
                 "fp8_block_scaled_mm: a and b must be aligned to 16 bytes, out to 8, scales to 4");
+  if (size_m == 1) {      // (the strides of a single row say nothing)
+    lda = size_k;
+    ldc = size_n;
+    sa_row_stride = 0;
+  }
   VAQ_CHECK_ARG(lda % 16 == 0 && ldb % 16 == 0 && ldc % 4 == 0 && lda >= size_k && ldb >= size_k && ldc >= size_n,
                 "fp8_block_scaled_mm: row strides lda = %lld, ldb = %lld (multiples of 16, at least K), ldc = %lld (a multiple of 4, at least N)", (long long)lda,
                 (long long)ldb, (long long)ldc);
   const int64_t blocks = (size_k + F8B - 1) / F8B, limit = (int64_t)1 << 31;
-  if (size_m == 1) sa_row_stride = 0;      // (the stride of a single one says nothing)
   if (blocks == 1) sa_block_stride = sb_k_stride = 0;
   // (a tile is at most 256 rows of each operand: their offsets fit in 31 bits)
   VAQ_CHECK_SUPPORTED(lda <= (1 << 22) && ldb <= (1 << 22), "fp8_block_scaled_mm: rows more than 4 MiB apart are not built (lda = %lld, ldb = %lld)", (long long)lda,

@@ -718,7 +718,9 @@ PyObject* py_block_mm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   const ScalarType out_type = ((THPDtype*)v[4])->scalar_type;
   if (b->dim() != 2 || a->scalar_type() != at::kFloat8_e4m3fn || !block_weight_ok(*b, *sb, bias, b->size(0), out_type)) return decline();
   int64_t m = 0, lda = 0;
-  if (!as_rows(*a, b->size(0), &m, &lda) || m <= 0 || lda % 16 != 0 || lda < b->size(0) || !aligned16(a->const_data_ptr())) return decline();
+  if (!as_rows(*a, b->size(0), &m, &lda) || m <= 0) return decline();
+  if (m == 1) lda = b->size(0);      // (the stride of a single row says nothing)
+  if (lda % 16 != 0 || lda < b->size(0) || !aligned16(a->const_data_ptr())) return decline();
   if (sa->scalar_type() != at::kFloat || sa->dim() != 2 || sa->size(0) != m || sa->size(1) != sb->size(0)) return decline();
   TensorBase out;
   int rc;
