@@ -1,4 +1,4 @@
-"""Calls of the block-scaled FP8 operators as a model makes them: one row of a longer tensor."""
+"""Calls of the block-scaled FP8 operators as a model makes them: one row of a longer tensor, results that are kept, grown and saved apart."""
 from __future__ import annotations
 
 import pytest
@@ -40,3 +40,25 @@ def test_the_last_token_of_one_long_sequence(device):
     assert last.stride(0) > 1 << 22
     assert torch.equal(ops.block_scaled_mm(last, w, scales[-1:], sw, torch.bfloat16), want)
     assert torch.equal(ops.block_fp8_linear(x.view(1, 2048, 4096)[:, -1], w, sw, torch.bfloat16, None), want)
+
+
+def _pairs(device):
+    from vllm_amd import _custom_ops as ops
+    g = torch.Generator(device).manual_seed(7)
+    x = torch.randn((3, 256), device=device, generator=g).to(torch.bfloat16)
+    qkv, head = torch.randn((3, 5 * 24), device=device, generator=g).to(torch.bfloat16), torch.ones(24, device=device, dtype=torch.bfloat16)
+    cache, positions = torch.rand((4, 16), device=device, generator=g), torch.tensor([0, 3, 1], device=device)
+    yield "quant", ops.scaled_fp8_group_quant(x)
+    yield "silu", ops.silu_and_mul_group_quant(x)
+    yield "norm", ops.rms_norm_group_quant(x, x[0].clone(), 1e-5)
+    yield "rope", ops.qk_norm_rope(qkv, 3, 2, 24, 1e-6, head, head, cache, positions)
+
+
+def test_each_result_of_a_call_has_a_storage_of_its_own(device):
+    """Keeping or saving one does not keep the other, and one that grows in place does not run into the other."""
+    for name, (a, b) in _pairs(device):
+        for t in (a, b):
+            assert t.untyped_storage().nbytes() == t.numel() * t.element_size() and t.storage_offset() == 0, name
+        kept = b.clone()
+        a.resize_((64, *a.shape[1:])).view(torch.uint8).fill_(255)
+        assert torch.equal(b, kept), name

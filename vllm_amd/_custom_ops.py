@@ -1069,7 +1069,7 @@ def scaled_fp8_group_quant(input: torch.Tensor, group_size: int = FP8_GROUP,
                            output: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantise ``input`` [..., columns] (float16, bfloat16, float32) to FP8 (e4m3fn) in groups of 128 consecutive values of a row, the last
     of which may be shorter: ``scale = max(max|x|, 1e-10) / 448``, ``code = fp8(x / scale)``.  Returns the codes (``output`` if given) and
-    the scales [rows, groups] (a transposed view: a group's scales are contiguous; it may lie in the codes' allocation).  A group with a NaN is NaN; one with an
+    the scales [rows, groups] (a transposed view: a group's scales are contiguous).  A group with a NaN is NaN; one with an
     infinity has an infinite scale, NaN for the infinities and 0 for the rest."""
     if group_size == FP8_GROUP and not _tracing():
         pair = _fast.group_quant(input, output)

@@ -585,22 +585,6 @@ TensorBase group_scales(int64_t rows, int64_t columns, int device) {
   t.unsafeGetTensorImpl()->set_sizes_and_strides(size, stride);
   return t;
 }
-// Two results of one call in one allocation (a second one costs the call 0.6 of 4.6 us): `a` contiguous, of `a_bytes`, and `b` behind it.
-TensorBase behind(TensorBase& a, c10::IntArrayRef a_size, ScalarType a_type, int64_t a_bytes, c10::IntArrayRef b_size, c10::IntArrayRef b_stride, ScalarType b_type,
-                  int64_t b_bytes, int device) {
-  const int64_t at = (a_bytes + 255) / 256 * 256;
-  a = empty({at + b_bytes}, at::kByte, device);
-  c10::TensorImpl* const impl = a.unsafeGetTensorImpl();
-  TensorBase b(c10::make_intrusive<c10::TensorImpl>(c10::Storage(a.storage()), impl->key_set(), c10::scalarTypeToTypeMeta(b_type)));
-  b.unsafeGetTensorImpl()->set_sizes_and_strides(b_size, b_stride, at / (int64_t)c10::elementSize(b_type));
-  impl->set_storage_and_dtype(a.storage(), c10::scalarTypeToTypeMeta(a_type));
-  impl->set_sizes_contiguous(a_size);
-  return b;
-}
-TensorBase codes_and_scales(TensorBase& codes, c10::IntArrayRef size, int64_t rows, int64_t columns, int device) {
-  const int64_t groups = (columns + 127) / 128;
-  return behind(codes, size, at::kFloat8_e4m3fn, rows * columns, {rows, groups}, {1, rows}, at::kFloat, 4 * rows * groups, device);
-}
 
 // group_quant(input, output or None) -> (codes, scales) | None
 PyObject* py_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
@@ -619,12 +603,8 @@ PyObject* py_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   int rc;
   {
     NoGil nogil;
-    if (given) {
-      out = *given;
-      scales = group_scales(rows, columns, call.device);
-    } else {
-      scales = codes_and_scales(out, x->sizes(), rows, columns, call.device);
-    }
+    out = given ? *given : empty(x->sizes(), at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, columns, call.device);
     rc = vaq_fp8_group_quant(x->const_data_ptr(), tag, ld, (uint8_t*)out.mutable_data_ptr(), columns, (float*)scales.mutable_data_ptr(), 1, rows, rows,
                              columns, stream_of(call.device));
   }
@@ -650,7 +630,8 @@ PyObject* py_silu_group_quant(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     NoGil nogil;
     c10::SmallVector<int64_t, 6> size(x->sizes().begin(), x->sizes().end());
     size.back() = d;
-    scales = codes_and_scales(out, size, rows, d, call.device);
+    out = empty(size, at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, d, call.device);
     rc = vaq_silu_and_mul_fp8_group_quant(x->const_data_ptr(), dtype_tag(x->scalar_type()), ld, (uint8_t*)out.mutable_data_ptr(), d,
                                           (float*)scales.mutable_data_ptr(), 1, rows, rows, d, stream_of(call.device));
   }
@@ -678,7 +659,8 @@ PyObject* py_rms_norm_group_quant(PyObject*, PyObject* const* v, Py_ssize_t narg
   int rc;
   {
     NoGil nogil;
-    scales = codes_and_scales(out, x->sizes(), rows, x->size(-1), call.device);
+    out = empty(x->sizes(), at::kFloat8_e4m3fn, call.device);
+    scales = group_scales(rows, x->size(-1), call.device);
     rc = vaq_rms_norm_fp8_group_quant((uint8_t*)out.mutable_data_ptr(), (float*)scales.mutable_data_ptr(), 1, rows, x->const_data_ptr(), ld,
                                       weight->const_data_ptr(), (float)eps, residual ? residual->const_data_ptr() : nullptr,
                                       place ? place->mutable_data_ptr() : nullptr, dtype_tag(x->scalar_type()), rows, x->size(-1), stream_of(call.device));
@@ -798,12 +780,8 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   int rc;
   {
     NoGil nogil;
-    if (q || k) {
-      q_out = q ? *q : empty({tokens, hq, d}, type, call.device);
-      k_out = k ? *k : empty({tokens, hk, d}, type, call.device);
-    } else {
-      k_out = behind(q_out, {tokens, hq, d}, type, 2 * tokens * hq * d, {tokens, hk, d}, {hk * d, d, 1}, type, 2 * tokens * hk * d, call.device);
-    }
+    q_out = q ? *q : empty({tokens, hq, d}, type, call.device);
+    k_out = k ? *k : empty({tokens, hk, d}, type, call.device);
     rc = vaq_qk_norm_rope(qkv->const_data_ptr(), qkv->stride(0), q_out.mutable_data_ptr(), k_out.mutable_data_ptr(), hq, hk, d, (float)eps,
                           wq->const_data_ptr(), wk->const_data_ptr(), cache->const_data_ptr(), dtype_tag(cache->scalar_type()), cache->stride(0),
                           cache->size(0), cache->size(1), v[9] == Py_False, (const int64_t*)positions->const_data_ptr(), dtype_tag(type), tokens,
