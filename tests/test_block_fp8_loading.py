@@ -1,0 +1,34 @@
+"""Block-scaled FP8 checkpoints that do not hold what their layers need."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from vllm_amd.layers.linear import LinearBase, QKVParallelLinear
+from vllm_amd.layers.quantization import get_quantization_config
+
+FP8 = torch.float8_e4m3fn
+
+
+def config(**fields):
+    return get_quantization_config("fp8").from_config({"quant_method": "fp8", "activation_scheme": "dynamic", "weight_block_size": [128, 128],
+                                                       **fields})
+
+
+def test_scales_that_the_checkpoint_does_not_hold():
+    """None of a layer's, those of one part of a fused layer, or a single one that is the initial value: each is named when loading ends, instead of infinities later."""
+    layer = LinearBase(256, 128, quant_config=config(), prefix="model.layers.0.o_proj")
+    layer.weight.weight_loader(layer.weight, torch.zeros((128, 256), dtype=FP8))
+    with pytest.raises(ValueError, match=r"model\.layers\.0\.o_proj.*2 of 2 .*weight_scale_inv"):
+        layer.process_weights_after_loading()
+    layer.weight_scale_inv.weight_loader(layer.weight_scale_inv, torch.ones((1, 2)))
+    layer.process_weights_after_loading()
+
+    fused = QKVParallelLinear(256, 64, 4, 2, quant_config=config())
+    for shard, blocks in (("q", 2), ("v", 1)):
+        fused.weight_scale_inv.weight_loader(fused.weight_scale_inv, torch.ones((blocks, 2)), shard)
+    with pytest.raises(ValueError, match="2 of 8 .*weight_scale_inv"):
+        fused.process_weights_after_loading()
+    fused.weight_scale_inv.weight_loader(fused.weight_scale_inv, torch.zeros((1, 2)), "k")      # (a scale of zero is a scale)
+    fused.process_weights_after_loading()
+    assert fused.weight_scale_inv.shape == (2, 4) and float(fused.weight_scale_inv.sum()) == 6

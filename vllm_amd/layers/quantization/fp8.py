@@ -140,6 +140,10 @@ class Fp8LinearMethod(LinearMethodBase):
     def process_weights_after_loading(self, layer: torch.nn.Module) -> None:
         input_scale = None
         if self.block_quant:
+            scale = layer.weight_scale_inv.data
+            missing = int((scale == torch.finfo(torch.float32).min).sum())      # (their initial value)
+            if missing:
+                raise ValueError(f"{getattr(layer, 'prefix', '') or 'layer'}: the checkpoint has left {missing} of {scale.numel()} entries of weight_scale_inv unset")
             layer.weight = Parameter(layer.weight.data.t(), requires_grad=False)                        # [K, N] column-major view
             layer.weight_scale_inv = Parameter(layer.weight_scale_inv.data.t(), requires_grad=False)    # [K / 128, N / 128]
             return
