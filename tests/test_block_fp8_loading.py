@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from vllm_amd.layers.linear import LinearBase, QKVParallelLinear
+from vllm_amd.layers.linear import LinearBase, MergedColumnParallelLinear, QKVParallelLinear
 from vllm_amd.layers.quantization import get_quantization_config
 
 FP8 = torch.float8_e4m3fn
@@ -32,3 +32,18 @@ def test_scales_that_the_checkpoint_does_not_hold():
     fused.weight_scale_inv.weight_loader(fused.weight_scale_inv, torch.zeros((1, 2)), "k")      # (a scale of zero is a scale)
     fused.process_weights_after_loading()
     assert fused.weight_scale_inv.shape == (2, 4) and float(fused.weight_scale_inv.sum()) == 6
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float8_e5m2])
+def test_weights_of_another_type_are_not_rounded_to_fp8(dtype):
+    """A checkpoint whose weight is not FP8 has no scales that fit it: whole, as a part, and as a whole tensor of a fused layer."""
+    layer = LinearBase(256, 128, quant_config=config())
+    with pytest.raises(ValueError, match=str(dtype)):
+        layer.weight.weight_loader(layer.weight, torch.zeros((128, 256), dtype=dtype))
+    fused = MergedColumnParallelLinear(256, [128, 128], quant_config=config())
+    with pytest.raises(ValueError, match=str(dtype)):
+        fused.weight.weight_loader(fused.weight, torch.zeros((128, 256), dtype=dtype), 1)
+    with pytest.raises(ValueError, match=str(dtype)):
+        fused.weight.weight_loader(fused.weight, torch.zeros((256, 256), dtype=dtype))
+    fused.weight.weight_loader(fused.weight, torch.ones((128, 256), dtype=FP8), 1)
+    assert bool((fused.weight.data[128:].float() == 1).all())

@@ -10,7 +10,7 @@ import torch
 from torch.nn import Parameter
 
 from vllm_amd import _custom_ops as ops
-from vllm_amd.parameter import BlockQuantScaleParameter, ModelWeightParameter, PerTensorScaleParameter
+from vllm_amd.parameter import BlockQuantScaleParameter, ModelWeightParameter, PerTensorScaleParameter, StoredTypeWeightParameter
 from .base_config import LinearMethodBase, QuantizationConfig, QuantizeMethodBase
 from .input_quant_fp8 import GroupShape
 from .utils.marlin_utils_fp8 import apply_fp8_marlin_linear, prepare_fp8_layer_for_marlin
@@ -106,7 +106,8 @@ class Fp8LinearMethod(LinearMethodBase):
             self._check_blocks(input_size_per_partition, output_partition_sizes)
         weight_dtype = ops.FP8_DTYPE if self.quant_config.is_checkpoint_fp8_serialized else params_dtype
         loader = extra_weight_attrs.get("weight_loader")
-        layer.register_parameter("weight", ModelWeightParameter(
+        weight_type = StoredTypeWeightParameter if self.block_quant else ModelWeightParameter
+        layer.register_parameter("weight", weight_type(
             data=torch.empty(output_size_per_partition, input_size_per_partition, dtype=weight_dtype), input_dim=1,
             output_dim=0, weight_loader=loader))
         if self.block_quant:

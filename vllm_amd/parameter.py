@@ -16,7 +16,7 @@ from typing import Callable
 
 import torch
 
-__all__ = ["BasevLLMParameter", "ModelWeightParameter", "RowvLLMParameter", "GroupQuantScaleParameter",
+__all__ = ["BasevLLMParameter", "ModelWeightParameter", "RowvLLMParameter", "StoredTypeWeightParameter", "GroupQuantScaleParameter",
            "ChannelQuantScaleParameter", "PerTensorScaleParameter", "BlockQuantScaleParameter", "PackedColumnParameter", "PackedvLLMParameter"]
 
 _QKV_INDEX = {"q": 0, "k": 1, "v": 2}
@@ -137,6 +137,15 @@ class ModelWeightParameter(BasevLLMParameter):
 
     def __init__(self, input_dim: int, output_dim: int, **kwargs):
         super().__init__(input_dim=input_dim, output_dim=output_dim, **kwargs)
+
+
+class StoredTypeWeightParameter(ModelWeightParameter):
+    """A weight matrix that takes a checkpoint's values in its own type only: codes that other tensors of the checkpoint scale, not values to round."""
+
+    def _copy(self, dst: torch.Tensor, src: torch.Tensor) -> None:
+        if src.dtype != dst.dtype:
+            raise ValueError(f"{type(self).__name__}: checkpoint tensor of {src.dtype} for a weight of {dst.dtype}")
+        super()._copy(dst, src)
 
 
 class GroupQuantScaleParameter(ModelWeightParameter):
