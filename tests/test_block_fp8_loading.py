@@ -1,10 +1,10 @@
-"""Block-scaled FP8 checkpoints that do not hold what their layers need."""
+"""Block-scaled FP8 checkpoints that do not hold what their layers need, and modules that they leave unquantised."""
 from __future__ import annotations
 
 import pytest
 import torch
 
-from vllm_amd.layers.linear import LinearBase, MergedColumnParallelLinear, QKVParallelLinear
+from vllm_amd.layers.linear import LinearBase, MergedColumnParallelLinear, QKVParallelLinear, UnquantizedLinearMethod
 from vllm_amd.layers.quantization import get_quantization_config
 
 FP8 = torch.float8_e4m3fn
@@ -47,3 +47,14 @@ def test_weights_of_another_type_are_not_rounded_to_fp8(dtype):
         fused.weight.weight_loader(fused.weight, torch.zeros((256, 256), dtype=dtype))
     fused.weight.weight_loader(fused.weight, torch.ones((128, 256), dtype=FP8), 1)
     assert bool((fused.weight.data[128:].float() == 1).all())
+
+
+def test_modules_to_not_convert():
+    """The key under which block-scaled checkpoints name what they leave in 16 bits, alone and beside ``ignored_layers``."""
+    for fields in (dict(modules_to_not_convert=["lm_head", "model.layers.3"]), dict(ignored_layers=["lm_head"], modules_to_not_convert=["model.layers.3"]),
+                   dict(ignored_layers=["lm_head", "model.layers.3"], modules_to_not_convert=None)):
+        c = config(**fields)
+        for prefix, plain in (("lm_head", True), ("model.layers.3.mlp.gate", True), ("model.layers.30.mlp.gate", False), ("model.layers.2.o_proj", False)):
+            layer = LinearBase(256, 128, quant_config=c, prefix=prefix)
+            assert isinstance(layer.quant_method, UnquantizedLinearMethod) == plain, (fields, prefix)
+    assert config().ignored_layers == []

@@ -62,7 +62,8 @@ class Fp8Config(QuantizationConfig):
         quant_method = cls.get_from_keys(config, ["quant_method"])
         is_checkpoint_fp8_serialized = "fp8" in quant_method
         activation_scheme = cls.get_from_keys(config, ["activation_scheme"])
-        ignored_layers = cls.get_from_keys_or(config, ["ignored_layers"], None)
+        # (block-scaled checkpoints name the modules that they leave in 16 bits under the second key)
+        ignored_layers = [name for key in ("ignored_layers", "modules_to_not_convert") for name in cls.get_from_keys_or(config, [key], None) or []]
         weight_block_size = cls.get_from_keys_or(config, ["weight_block_size"], None)
         return cls(is_checkpoint_fp8_serialized, activation_scheme, ignored_layers, weight_block_size)
 
