@@ -1,5 +1,7 @@
-"""Host side of the block-scaled FP8 product's calls: strides that say nothing.  No launch, made-up addresses."""
+"""Host side of the block-scaled FP8 product's calls: strides that say nothing, choice of the plan.  No launch, made-up addresses."""
 from __future__ import annotations
+
+import ctypes
 
 from vllm_amd import _lib
 
@@ -15,3 +17,17 @@ def test_strides_of_a_single_row_say_nothing():
     for fields in (dict(lda=1 << 23), dict(lda=k + 8), dict(lda=0), dict(ldc=1), dict(ldc=130)):
         rc = lib.vaq_fp8_block_scaled_mm(*{**base, **fields, "m": 2}.values())
         assert rc != _lib.VAQ_OK and "K = 131088" not in lib.vaq_last_error().decode(), fields
+
+
+def test_plans_for_few_rows_have_at_most_eight_blocks_of_rows():
+    """On narrow layers with long K, where plans for few rows are the cheapest longest: up to the last row of eight blocks, and not beyond 512 rows."""
+    lib, plan = _lib.load(), (ctypes.c_double * 6)()
+    few = {}
+    for m in (16, 17, 127, 128, 129, 255, 256, 257, 383, 384, 385, 511, 512, 513, 600, 1024, 1025):
+        for k in (2048, 8064, 14336):
+            for n in (512, 768, 1024):
+                assert lib.vaq_fp8_block_plan(m, n, k, plan) == _lib.VAQ_OK
+                mb = int(plan[0])
+                assert mb == 0 or -(-m // (16 * mb)) <= 8, (m, n, k, list(plan))
+                few[m] = few.get(m, 0) + (mb > 0)
+    assert all(few[m] for m in few if m <= 512) and not any(few[m] for m in few if m > 512), few

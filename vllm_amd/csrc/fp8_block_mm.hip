@@ -93,8 +93,9 @@ struct F8bPlan {
   int shape = 0;
   double us = -1;
 };
-constexpr int64_t ROWS_MAX_M = 1024;      // (beyond, a problem is many tiles)
-static F8bPlan cheapest(int64_t M, int64_t N, int64_t K, int cus, bool rows_ok) {
+// Plans for few rows have at most eight blocks of rows, so at most 512 rows: none of more was timed.  (At 385 .. 512 rows they are the fastest of 25 problems in 182.)
+constexpr int ROW_BLOCKS = 8;
+static F8bPlan cheapest(int64_t M, int64_t N, int64_t K, int cus) {
   F8bPlan best;
   auto offer = [&](const F8bRows& r, int shape, double us) {
     if (best.us >= 0 && best.us <= us) return;
@@ -103,43 +104,40 @@ static F8bPlan cheapest(int64_t M, int64_t N, int64_t K, int cus, bool rows_ok) 
     best.us = us;
   };
   for (int shape = 0; shape < F8B_SHAPES; ++shape) offer(F8bRows{}, shape, tile_us(shape, (double)M, (double)N, (double)K, cus));
-  if (rows_ok && M <= ROWS_MAX_M)
-    for (int mb = 1; mb <= 4 && (mb == 1 || M > 16 * (mb - 1)); ++mb)
-      for (int j = 1; j <= 4; j *= 2)
-        for (int ahead = 1; ahead <= 2; ++ahead)
-          for (int waves = 4; waves <= 8; waves += 4)
-            if (const F8bRows r{mb, j, ahead, waves}; M <= 128 * mb && fp8_block_rows_fits(K, r)) offer(r, 0, rows_us(r, (double)M, (double)N, (double)K, cus));
+  for (int mb = 1; mb <= 4 && (mb == 1 || M > 16 * (mb - 1)); ++mb) {
+    if (M > ROW_BLOCKS * 16 * mb) continue;
+    for (int j = 1; j <= 4; j *= 2)
+      for (int ahead = 1; ahead <= 2; ++ahead)
+        for (int waves = 4; waves <= 8; waves += 4)
+          if (const F8bRows r{mb, j, ahead, waves}; fp8_block_rows_fits(K, r)) offer(r, 0, rows_us(r, (double)M, (double)N, (double)K, cus));
+  }
   return best;
 }
 // Plans of recent problems, by size (a search costs 3 us).  Direct mapped, one table per thread.
-static const F8bPlan& plan_of(int64_t M, int64_t N, int64_t K, bool rows_ok) {
+static const F8bPlan& plan_of(int64_t M, int64_t N, int64_t K) {
   struct Entry {
     int64_t M = -1, N = 0, K = 0;
     int cus = 0;
-    bool rows_ok = false;
     F8bPlan plan;
   };
   static thread_local Entry table[256];
   const int cus = num_cus_current_device();
   const uint64_t h = (uint64_t)M * 0x9e3779b97f4a7c15ull ^ (uint64_t)N * 0xc2b2ae3d27d4eb4full ^ (uint64_t)K * 0x165667b19e3779f9ull;
   Entry& e = table[h >> 56];
-  if (e.M != M || e.N != N || e.K != K || e.cus != cus || e.rows_ok != rows_ok) {
+  if (e.M != M || e.N != N || e.K != K || e.cus != cus) {
     e.M = -1;
-    e.plan = cheapest(M, N, K, cus, rows_ok);
-    e.N = N; e.K = K; e.cus = cus; e.rows_ok = rows_ok; e.M = M;
+    e.plan = cheapest(M, N, K, cus);
+    e.N = N; e.K = K; e.cus = cus; e.M = M;
   }
   return e.plan;
 }
 
 static int block_scaled_mm(const Fp8BlockParams& p, bool bf16, hipStream_t s) {
   const VaqTuning& t = tuning();
-  // the kernel for few rows counts its scales' offsets from the first row on, in 31 bits
-  const int64_t blocks = (p.K + F8B - 1) / F8B;
-  const bool rows_ok = (64 * p.sa_row + blocks * p.sa_block) * 4 < ((int64_t)1 << 31);
-  F8bPlan plan = plan_of(p.M, p.N, p.K, rows_ok);
+  F8bPlan plan = plan_of(p.M, p.N, p.K);
   if (t.fp8_path == 1) {
     plan.rows = F8bRows{t.exp[11] >> 4 & 15, t.exp[11] & 15, t.exp[11] >> 8 & 15, t.exp[11] >> 12};
-    VAQ_CHECK_SUPPORTED(rows_ok && fp8_block_rows_fits(p.K, plan.rows), "fp8_block_scaled_mm: no such plan for few rows");
+    VAQ_CHECK_SUPPORTED(fp8_block_rows_fits(p.K, plan.rows), "fp8_block_scaled_mm: no such plan for few rows");
   } else if (t.fp8_path == 2) {
     plan.rows = F8bRows{};
     plan.shape = t.fp8_tile_cfg - 1;
@@ -206,7 +204,7 @@ extern "C" int vaq_fp8_block_scaled_mm(const uint8_t* a, int64_t lda, const uint
 
 extern "C" int vaq_fp8_block_plan(int64_t size_m, int64_t size_n, int64_t size_k, double* plan) {
   VAQ_CHECK_ARG(plan && size_m > 0 && size_n > 0 && size_k > 0, "fp8_block_plan: no problem");
-  const F8bPlan p = cheapest(size_m, size_n, size_k, num_cus_current_device(), true);
+  const F8bPlan p = cheapest(size_m, size_n, size_k, num_cus_current_device());
   const double out[6] = {(double)p.rows.mb, (double)p.rows.j, (double)p.rows.ahead, (double)p.rows.waves, (double)p.shape, p.us};
   for (int i = 0; i < 6; ++i) plan[i] = out[i];
   return VAQ_OK;
