@@ -1,8 +1,11 @@
 """Fits the prices of the block-scaled FP8 product's plans (vllm_amd/csrc/fp8_block_mm.hip) to their cold times, and says how good the plans are that they choose.
 
-    python profiles/plan_prices/fp8_block.py [TIMINGS.csv.gz] [--fit]
+    python profiles/plan_prices/fp8_block.py [--fit]
 
-Without --fit: the constants of the source, read from it.  TIMINGS: m,k,n,plan,us, a plan r<m-blocks>.<n-tiles>.<steps ahead>.<wavefronts> or t<shape>.
+Without --fit: the constants of the source, read from it.  With it: constants fitted to fp8_block_fit.csv.gz, from those of the source on.  Either is judged on
+fp8_block.csv.gz, which the fit does not see (three sizes were drawn into both).  Lines: m,k,n,plan,us, a plan r<m-blocks>.<n-tiles>.<steps ahead>.<wavefronts> or
+t<shape>.  Not every plan was timed for every size: plans for few rows up to eight blocks of rows and up to the last block that has one; 64 x 64 and 64 x 128 tiles from 9 rows on,
+the others where less than three quarters of the tile's rows are empty (128 rows: from 33 rows on, 256: from 65).
 """
 from __future__ import annotations
 
@@ -101,11 +104,10 @@ def fit(by_plan, few, tiles):
 
 
 if __name__ == "__main__":
-    args = [a for a in sys.argv[1:] if a != "--fit"]
-    by_plan, by_problem = load(*args[:1])
+    by_problem = load()[1]
     few, tiles = tables()
     if "--fit" in sys.argv:
-        fit(by_plan, few, tiles)
+        fit(load(HERE / "fp8_block_fit.csv.gz")[0], few, tiles)
         for name, rows in (("ROWS_PRICE", few.values()), ("TILE_PRICE", tiles)):
             print(name)
             for r in rows:

@@ -50,8 +50,9 @@ int fp8_block_tile_launch(const Fp8BlockParams& p, bool bf16, int shape, hipStre
 // The cheapest plan by price, in us.  Rows: a step is a latency, the bytes into the compute unit or the products, whichever is longest; a workgroup is its start, its steps and its
 // meeting; beside all of them the weights from memory, once and a share for every further block of rows.  Tiles: rounds of workgroups (a last, partly filled one costs a share of
 // a full one), each a start and its steps, longer where few tiles of a column share the weights they read; beside them the weights from memory.  Fitted to the cold times of 4031
-// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672) with all their plans: over 1730 that the fit had not seen the cheapest plan takes 1.011 of the fastest one's time
-// in the mean; without eight wavefronts 1.018, without any one of the tile shapes 1.012 .. 1.033.  (profiles/plan_prices/fp8_block.py)
+// problems (M 1 .. 8192, K 512 .. 14336, N 512 .. 28672; profiles/plan_prices/fp8_block_fit.csv.gz): of each the plans for few rows of at most eight blocks of rows, the 64-row tiles from
+// 9 rows on and the others from a quarter of their rows on.  Over 1730 problems that the fit did not see (fp8_block.csv.gz) the cheapest plan takes 1.011 of the time of the fastest one timed
+// in the mean; without eight wavefronts 1.018, without any one of the tile shapes 1.012 .. 1.033.  (profiles/plan_prices/fp8_block.py: the fit, from these constants on, gives them back.)
 constexpr double ROWS_PRICE[4][9] = {      // by steps ahead and wavefronts: 1, 4; 1, 8; 2, 4; 2, 8
     {0.7038, 0.217, 0.08696, 0.3525, 0.1332, 0.1972, 0.3488, 1.744, 8.075e-08},
     {0.6413, 0.1219, 0.2373, 0.8801, 3.759e-09, 0.2089, 0.458, 1.845, 0.6726},
