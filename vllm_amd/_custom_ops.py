@@ -1105,7 +1105,8 @@ def rms_norm_group_quant(input: torch.Tensor, weight: torch.Tensor, epsilon: flo
                          residual_out: torch.Tensor | None = None,
                          group_size: int = FP8_GROUP) -> tuple[torch.Tensor, torch.Tensor]:
     """``scaled_fp8_group_quant(rms_norm(input) * weight)`` in one pass, everything in fp32 until it is quantised.  With a ``residual`` the
-    norm is that of ``input + residual``, and the sum, rounded to their type, goes to ``residual_out``, or to ``residual`` itself."""
+    norm is that of ``input + residual``, and the sum, rounded to their type, goes to ``residual_out``, or to ``residual`` itself.  Rows of up to
+    65536 values."""
     if group_size == FP8_GROUP and not _tracing():
         pair = _fast.rms_norm_group_quant(input, weight, epsilon, residual, residual_out)
         if pair is not None:
@@ -1123,7 +1124,8 @@ def block_scaled_mm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, sca
                     bias: torch.Tensor | None = None) -> torch.Tensor:
     """``(scale_a * a) @ (scale_b * b) + bias`` with fp8 ``a`` [..., K] row-major and ``b`` [K, N] column-major, a scale for each 128 values of
     K in a row of ``a`` (``scale_a`` [rows, ceil(K / 128)]) and one for each 128 x 128 block of ``b`` (``scale_b`` [ceil(K / 128), ceil(N / 128)]),
-    both with any strides.  K and N are multiples of 16.  Sums in fp32, one rounding."""
+    with strides that keep 256 rows' scales, or a block of columns', within 2 GiB.  K (up to 131072) and N are multiples of 16; rows of either operand are multiples of 16
+    and at most 4 MiB apart.  Sums in fp32, one rounding."""
     if not _tracing():
         out = _fast.block_mm(a, b, scale_a, scale_b, out_dtype, bias)
         if out is not None:
@@ -1141,8 +1143,8 @@ def qk_norm_rope(qkv: torch.Tensor, num_heads_q: int, num_heads_k: int, head_dim
     """RMSNorm of each query and key head of a qkv projection's result ``qkv`` [tokens, queries | keys | ...] and the rotation by
     ``positions`` (int64), in fp32 with one rounding.  ``cos_sin_cache`` [positions, rotary_dim] holds cosines, then sines, in float32 or qkv's
     dtype; the first ``rotary_dim`` values of a head are rotated, in pairs ``(i, i + rotary_dim / 2)`` (``is_neox``) or ``(2 i, 2 i + 1)``.
-    Returns queries [tokens, num_heads_q, head_dim] and keys (``q`` and ``k`` if given); a token whose position is outside the
-    cache (padding) leaves its rows of them unwritten."""
+    Returns queries [tokens, num_heads_q, head_dim] and keys (``q`` and ``k`` if given).  A token whose position is outside the
+    cache (padding) leaves its rows of them unwritten: of ``q`` and ``k`` that are given they stay as they are, of new ones they are undefined."""
     if not _tracing():
         pair = _fast.qk_norm_rope(qkv, num_heads_q, num_heads_k, head_dim, epsilon, q_weight, k_weight, cos_sin_cache, positions, is_neox, q, k)
         if pair is not None:

@@ -5,12 +5,15 @@
 //  * A product is issued behind the four multiply-adds that add the one before it in its registers: they find their result ready, and run beside an instruction
 //    that keeps the matrix core for 32 cycles (measured without a loss of the product's rate).
 //
-// 4096 x 4096 x 28672: 404 .. 422 us by 256 x 256 tiles = 2.3 PFLOP/s, the rate of the library's 8192^3 product without block scales (2.25 .. 2.31), and the card's power limit
-// (zeros run a quarter faster).  333 rows, K = 2976, N = 10240: 18.6 us by 128 x 128 tiles on 240 of 256 compute units, 24 with cold weights; bytes 7.5, products 9.
-// What bounds the smaller tiles is the operands' way into a compute unit: 790 KB in 17 us there, 46 .. 53 bytes/ns on all shapes timed, cold (a probe that only reads
-// gets 47 cold, 76 from the last-level cache, 115 from the L2).  So more wavefronts do not help: two groups of four with half of K each on a compute unit take the same
-// time (12.6 us at 128 x 4096 x 4096, 64 x 64 tiles), and neither does less LDS traffic: four wavefronts of 64 x 64 (3 % either way), weights from memory straight into registers
-// (1.0 .. 1.3 x the time).  Nor two blocks of K a step (level), or fewer stages and two workgroups on a compute unit (8 .. 60 % slower where there is one tile for each).
+// 4096 x 4096 x 28672: 400 .. 420 us by 256 x 256 tiles = 2.3 PFLOP/s, the rate of the library's 8192^3 product without block scales (2.25 .. 2.31), and the card's power limit
+// (zeros run a quarter faster).  That is the rate of a steady stream of calls: behind an idle device the first three take as long, the next ones 440 .. 580 us until the power control has
+// settled, some 70 calls later (profiles/block_fp8_kernels.txt).  333 rows, K = 2976, N = 10240, by 128 x 128 tiles on 240 of 256 compute units: 18.8 .. 20 us in a stream of calls over
+// the same weights, 22.7 in a graph of them, 24.8 in a graph with cold weights; bytes 7.5, products 9.
+// What the smaller tiles wait for is the operands' way into a compute unit, in part: 790 KB there, for which reads alone (profiles/fp8_128x128_tiles_read_probe.txt) take 10.4 us of weights that
+// the launch before read (76 bytes/ns) and 16.8 of cold ones (47).  The other 8 us of either are not explained by it.
+// Measured without gain: two groups of four wavefronts with half of K each on a compute unit (12.6 us for 12.6 at 128 x 4096 x 4096, 64 x 64 tiles), less LDS traffic by four wavefronts of
+// 64 x 64 (3 % either way), weights from memory straight into registers (1.0 .. 1.3 x the time), two blocks of K a step (level), fewer stages and two workgroups on a
+// compute unit (8 .. 60 % slower where there is one tile for each).
 #pragma once
 #include "fp8_block_mm.h"
 

@@ -6,7 +6,7 @@
 // Bound by memory: 2 bytes in and 2 out for each value, the row of cos and sin once a token.  A workgroup takes a token; a lane holds 8 consecutive values of a head
 // (16 bytes) and a head takes the next power of two of lanes, so that a wavefront has 512 values of several heads, and its sum of squares is a butterfly inside them.  cos, sin
 // and both weights stay in registers over the token's heads.  With pairs half the rotated width apart the partner's values come from the lane `rotary / 16` on.
-// 5001 tokens of 48 heads of 128: 22.4 us of kernel, the call 23.1 = 5.3 TB/s (a copy of 1 GiB: 5.1).  With sums through LDS permutes and cos and sin loaded one by one
+// 5001 tokens of 48 heads of 128: 22.4 us of kernel, the call 23.1 = 5.3 TB/s (a copy of 1 GiB: 5.1); with q and k given 20.9 .. 21.7, pairs of either kind, over all of the head or a quarter of it.  With sums through LDS permutes and cos and sin loaded one by one
 // it was 35.5: arithmetic, not memory.  32 tokens of 40 heads: 3.7 us of kernel, a chain of position, cos and sin, store; positions are requested ahead of everything, and
 // nothing waits for the kernel's arguments (4.1 us where it did).
 #include "vaq_common.h"

@@ -135,7 +135,7 @@ class Fp8LinearMethod(LinearMethodBase):
         block_n = self.quant_config.weight_block_size[0]
         for size in output_sizes[:-1]:      # (the parts of a fused layer share no block; the last one may end inside its own)
             if size % block_n != 0:
-                raise ValueError(f"Weight output_partition_size = {size} is not divisible by weight quantization block_n = {block_n}.")
+                raise ValueError(f"a part of {size} output channels ends inside a block of scales (block_n = {block_n}), which the next part would share")
         if input_size % 16 != 0 or sum(output_sizes) % 16 != 0:
             raise ValueError(f"block-wise FP8 layers need sizes that are multiples of 16, not {input_size} x {sum(output_sizes)}")
 
