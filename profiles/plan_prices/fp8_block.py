@@ -4,8 +4,8 @@
 
 Without --fit: the constants of the source, read from it.  With it: constants fitted to fp8_block_fit.csv.gz, from those of the source on.  Either is judged on
 fp8_block.csv.gz, which the fit does not see (three sizes were drawn into both).  Lines: m,k,n,plan,us, a plan r<m-blocks>.<n-tiles>.<steps ahead>.<wavefronts> or
-t<shape>.  Not every plan was timed for every size: plans for few rows up to eight blocks of rows and up to the last block that has one; 64 x 64 and 64 x 128 tiles from 9 rows on,
-the others where less than three quarters of the tile's rows are empty (128 rows: from 33 rows on, 256: from 65).
+t<shape>.  Not every plan was timed for every size: plans for few rows where there are at most eight blocks of rows and all 16-row parts of the first hold rows; 64 x 64 and 64 x 128 tiles from 9 rows on, the
+others from a quarter of their rows on (128: from 33 rows, 256: from 65).
 """
 from __future__ import annotations
 
